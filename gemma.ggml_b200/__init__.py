@@ -23,6 +23,7 @@ HEADER = os.path.join(ROOT, "include", "ggml_b200.h")
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0 = 0, 1, 2, 8
 TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K = 12, 14, 15
 TYPE_BF16 = 30
+KV8_INT8, KV8_E4M3 = 1, 2  # codes of the 8-bit cache
 DTYPES = {"bfloat16": TYPE_BF16, "float32": TYPE_F32}
 BLOCK_BYTES = {TYPE_Q4_0: 18, TYPE_Q8_0: 34}
 
@@ -207,6 +208,10 @@ _CUDA_SIG = {
     "ggb_op_masked_attn_gated": (i32, [i32, vp, vp, vp, i32, vp, i64, i32, i32, i32, i32, i64, i64, f32, vp, vp, i64, vp, vp]),
     "ggb_op_moe_route_softmax_groups": (i32, [i32, vp, i64, i64, vp, vp, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp]),
     "ggb_op_moe_linear_shared": (i32, [i32, vp, i64, i64, vp, i64, i32, i64, i32, i32, vp, i32, vp, i64, vp, i64, i64, vp, i64, vp]),
+    "ggb_kv8_page_bytes": (i64, [i32, i32, i32, i32]), "ggb_kv8_attn_scratch_bytes": (sz, [i32]), "ggb_draft_verify_scratch_bytes": (sz, [i64, i32]),
+    "ggb_op_kv8_store": (i32, [i32, vp, vp, vp, i64, i64, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp, f32, vp, i64, i32, vp, vp]),
+    "ggb_op_kv8_attn": (i32, [i32, i32, vp, vp, vp, i64, i32, i64, i64, i32, vp, vp, i32, i32, i32, i32, i64, i64, f32, vp, vp, i64, vp, vp, sz]),
+    "ggb_op_draft_verify": (i32, [vp, i64, vp, i64, i64, i64, i32, vp, vp, vp, f32, vp, vp, vp, sz]),
     "ggb_comm_unique_id": (i32, [vp]), "ggb_comm_init": (i32, [vp, i32, i32]), "ggb_comm_destroy": (i32, []),
     "ggb_comm_rank": (i32, []), "ggb_comm_size": (i32, []), "ggb_op_allgather": (i32, [vp, vp, sz]),
 }

@@ -493,6 +493,50 @@ int ggb_op_diff_attn(int dt, const float *q, const void *cache, const int32_t *b
                      int G, int D, int Dv, int64_t window, int64_t keep_first, float softcap, float lambda, float out_scale, float eps,
                      const float *gate, int64_t ldg, void *out, float *scratch);
 
+/* ------------------------------------------------------------------ 8-bit paged cache of a batch (csrc/kv8_store.cu, csrc/kv8_attention.cu)
+ * A page of block_size positions (a multiple of 16) holds for each of the G key heads a record: codes of the keys [block_size][D], of the
+ * values [block_size][Dv], fp32 scales of the keys [block_size / 16] and of the values [block_size / 16], in whole 128 bytes (page j of the cache
+ * begins at j * ggb_kv8_page_bytes(...); 0 for sizes that no operator takes).  A number is its code times the scale of its group: 16 consecutive
+ * positions (from a multiple of 16 on) of one head.  D and Dv: multiples of 16 up to 256.
+ *
+ * A batch: sequence s < n_seq brings the tokens starts[s] .. starts[s + 1] - 1 (starts[0] = 0; none at all where the two are equal), which take the
+ * positions pos0[s], pos0[s] + 1, ...; position j lies in page tables[s * table_ld + j / block_size].  starts, pos0 and tables are device int32 (a captured call
+ * replays elsewhere); T is the rows that the buffers hold, and rows behind starts[n_seq] are neither read nor written.  The sequences of a call write to
+ * pages of their own; a table's entries outside of what a sequence sees and brings are not read. */
+#define GGB_KV8_INT8 1 /* codes -127 .. 127 */
+#define GGB_KV8_E4M3 2 /* 8-bit floating point, up to 448 */
+int64_t ggb_kv8_page_bytes(int G, int D, int Dv, int block_size);
+/* q [T][H * D], k [T][G * D], v [T][G * Dv] raw projections (fp32, row stride ld).  The pairs of the first rot_dims numbers of every head of q and k are turned by
+ * the position (cos_sin [positions][rot_dims / 2][2], rot_halves as for ggb_op_masked_qkv_store); q times scale -> q_out fp32 [T][H * D]; k and v -> the cache.
+ * A group's scale: with least = max|x| over its new tokens / (127 or 448) (at least 2^-100 unless all are zero) and old = its scale where it holds tokens before pos0
+ * (else 0), it is old where least <= old and otherwise max(least, 2 old), and the codes that it holds are rounded anew, to the nearest (ties to even), from code * (old /
+ * new).  New codes: x * (1 / scale), rounded so.  NaN is kept as 0 and infinities as the largest code; neither counts in max|x|.  Tokens that are written again (a
+ * draft that did not stand) take the place of what was there. */
+int ggb_op_kv8_store(int code, const float *q, const float *k, const float *v, int64_t ld, int64_t T, int n_seq, const int32_t *starts, const int32_t *pos0, int H,
+                     int G, int D, int Dv, int rot_dims, int rot_halves, const float *cos_sin, float scale, const int32_t *tables, int64_t table_ld, int block_size,
+                     void *cache, float *q_out);
+/* Soft-max attention of q (fp32 [T][H * D], as ggb_op_kv8_store leaves it) over the cache, the batch's own new tokens in it: the query at position i sees j <= i, with
+ * window > 0 only i - j < window or j < keep_first; softcap, sink (fp32 [H] or NULL) and gate (fp32 rows of stride ldg or NULL) as for ggb_op_masked_attn_gated; query
+ * head h reads key head h / (H / G).  out (dt) [T][H * Dv].  max_new: no sequence brings more tokens than that.  A query that is not finite makes its own row NaN.
+ * scratch (16-byte boundary, ggb_kv8_attn_scratch_bytes; NULL: none) lets the keys of a few rows be spread over many CTAs. */
+size_t ggb_kv8_attn_scratch_bytes(int Dv);
+int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const int32_t *tables, int64_t table_ld, int block_size, int64_t T, int64_t max_new,
+                    int n_seq, const int32_t *starts, const int32_t *pos0, int H, int G, int D, int Dv, int64_t window, int64_t keep_first, float softcap,
+                    const float *sink, const float *gate, int64_t ldg, void *out, void *scratch, size_t scratch_bytes);
+
+/* ------------------------------------------------------------------ drafted tokens (csrc/draft_verify.cu)
+ * Sequence s has the rows starts[s] .. starts[s + 1] - 1 (device int32; R: rows that the buffers hold, those behind starts[n_seq] stay as they were) of target logits
+ * (fp32, V numbers, stride ld_target); row j of them follows j drafted tokens, and every row but the last judges the token drafted[row].  p = soft-max(target /
+ * temperature), q = soft-max(draft / temperature) (draft NULL: 1 at the drafted token).  The token d of a row stands where u[row] q(d) < p(d); n_accepted[s] stand before
+ * the first that does not.  Behind them one is drawn: of the row where a draft fell from max(p - q, 0) over its sum (should that be nothing: from p), of the last
+ * row where all stand from p: the first v where the running sum exceeds u[last row] times the whole.  temperature 0: a token stands where it is the first maximum, which
+ * is also drawn (draft and u are not read).  tokens[starts[s] + j]: the tokens that stand, the drawn one, then -1.  Logits of -inf have probability 0; a row with NaN or
+ * +inf (temperature 0: with NaN), or with nothing above -inf, has no distribution: no token stands by it and -1 is drawn.  A drafted token outside of [0, V) falls.
+ * scratch: ggb_draft_verify_scratch_bytes, on a 16-byte boundary. */
+size_t ggb_draft_verify_scratch_bytes(int64_t R, int n_seq);
+int ggb_op_draft_verify(const float *target, int64_t ld_target, const float *draft, int64_t ld_draft, int64_t V, int64_t R, int n_seq, const int32_t *starts,
+                        const int32_t *drafted, const float *u, float temperature, int32_t *tokens, int32_t *n_accepted, void *scratch, size_t scratch_bytes);
+
 /* ------------------------------------------------------------------ sigmoid attention (csrc/sigmoid_attention.cu)
  * Grouped-query attention with unnormalised weights over the same paged rows [k (G * D) | v (G * Dv)] (ggb_window_cache_ld):
  * the weight of key j for the query at position i is sigmoid(q . k - r1[h] ln(1 + r2[h] (i - j)) + pb[h]), the output
