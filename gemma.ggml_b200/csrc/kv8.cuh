@@ -5,10 +5,12 @@
 // group: 16 consecutive positions of one head, keys and values apart.
 #pragma once
 
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <stdint.h>
 
-#include "common.cuh"
+#include "dense.cuh"
+#include "tc.cuh"
 
 constexpr int kKv8Group = 16;    // positions that share a scale
 constexpr int kKv8MaxHead = 256; // numbers of a key or value
@@ -47,4 +49,63 @@ template <> struct kv8_code<GGB_KV8_E4M3> {
     }
     __device__ static __forceinline__ uint8_t encode(float y) { return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3); }
 };
+
+namespace kv8 {
+
+struct attn_args {
+    const float *q;
+    const uint8_t *cache;
+    const int32_t *tables;
+    int64_t table_ld;
+    int B, n_seq;
+    const int32_t *starts, *pos0;
+    int H, G, D, Dv;
+    int64_t window, keep;
+    float cap;
+    const float *sink, *gate;
+    int64_t ldg, record;
+    void *out;
+    int groups;     // items of a sequence and key head, at most
+    float *part;    // [CTA][2][rows][Dv + 2], or null: an item a CTA
+    int4 *desc;     // [CTA]: sequence (or -1), group of rows, key head, last CTA of the item that begins here and ends elsewhere
+    int vec_q;      // queries begin on a 16-byte boundary
+};
+// four codes as two pairs of fp16 numbers.  int8: code + 128 behind the bits of 1024, less 1152
+template <int CODE> __device__ __forceinline__ void halves_of(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if (CODE == GGB_KV8_INT8) {
+        w ^= 0x80808080u;
+        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+    } else {
+        asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+    }
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2 *>(&h)); }
+
+// a power of two that brings m to [2^10, 2^11); 1 for zero and what is not finite
+__device__ __forceinline__ float to_half_range(float m) {
+    const int e = (int)(__float_as_uint(m) >> 23) - 127;
+    return e == 128 || m == 0.f ? 1.f : __uint_as_float((uint32_t)(min(max(10 - e, -126), 126) + 127) << 23);
+}
+
+// a row's sums, relative to 2^m, over the denominator (with the sink), times the gate
+struct row_end {
+    float f; // what the sums are multiplied by
+    __device__ __forceinline__ row_end(const attn_args &a, int h, float m, float l) {
+        if (a.sink) {
+            const float s = a.sink[h], M = fmaxf(m, s * kLog2e), c = m == -INFINITY ? 0.f : exp2f(m - M);
+            f = c / fmaf(l, c, s == -INFINITY ? 0.f : exp2f(fmaf(s, kLog2e, fmaf(s, kLog2eRest, -M))));
+        } else {
+            f = 1.f / l;
+        }
+    }
+};
+__device__ __forceinline__ float gated(const attn_args &a, float y, int64_t t, int64_t at) { return a.gate ? y / (1.f + expf(-a.gate[t * a.ldg + at])) : y; }
+
+} // namespace kv8
 #endif
