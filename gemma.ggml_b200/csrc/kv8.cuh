@@ -69,6 +69,7 @@ struct attn_args {
     float *part;    // [CTA][2][rows][Dv + 2], or null: an item a CTA
     int4 *desc;     // [CTA]: sequence (or -1), group of rows, key head, last CTA of the item that begins here and ends elsewhere
     int vec_q;      // queries begin on a 16-byte boundary
+    int *wait_error;
 };
 // four codes as two pairs of fp16 numbers.  int8: code + 128 behind the bits of 1024, less 1152
 template <int CODE> __device__ __forceinline__ void halves_of(uint32_t w, uint32_t &lo, uint32_t &hi) {
@@ -87,10 +88,10 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
 }
 __device__ __forceinline__ float2 half2_floats(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2 *>(&h)); }
 
-// a power of two that brings m to [2^10, 2^11); 1 for zero and what is not finite
-__device__ __forceinline__ float to_half_range(float m) {
+// a power of two that brings m to [2^to, 2^(to + 1)); 1 for zero
+__device__ __forceinline__ float power_for(float m, int to) {
     const int e = (int)(__float_as_uint(m) >> 23) - 127;
-    return e == 128 || m == 0.f ? 1.f : __uint_as_float((uint32_t)(min(max(10 - e, -126), 126) + 127) << 23);
+    return m == 0.f ? 1.f : __uint_as_float((uint32_t)(min(max(to - e, -126), 126) + 127) << 23);
 }
 
 // a row's sums, relative to 2^m, over the denominator (with the sink), times the gate

@@ -21,6 +21,8 @@
 #include <algorithm>
 #include <type_traits>
 
+#include <cuda.h>
+
 #include "kv8.cuh"
 
 namespace {
@@ -60,17 +62,51 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+__device__ __forceinline__ uint4 lds_u4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds_u2(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+// the cache as lines of 128 bytes (a record is whole lines, and 16 rows of it are): boxes of a group's keys and of its values, piece c of line l of a box at place
+// c ^ (l & 7), so that a quarter of a warp reads pieces of several rows from different banks
+struct line_maps {
+    CUtensorMap k, v;
+};
+__device__ __forceinline__ void request(const line_maps &m, uint32_t k_dst, uint32_t v_dst, int k_line, int v_line, uint32_t bytes, uint32_t bar) { // one lane
+    mbar_expect_tx(bar, bytes);
+    tma_load_2d(k_dst, &m.k, 0, k_line, bar);
+    tma_load_2d(v_dst, &m.v, 0, v_line, bar);
+}
+__device__ __forceinline__ uint32_t in_box(int byte) { return (uint32_t)(byte & ~127) + ((((byte >> 4) & 7) ^ ((byte >> 7) & 7)) << 4) + (byte & 15); }
+
 // P: numbers of a key and of a value, at most: 64, 128 or 256
-template <int P, int NT, int PARTS> struct step_sizes {
-    static constexpr int R = 8 * NT, KS = P / 16; // MMA steps along a key; blocks of 16 value coordinates
-    static constexpr size_t q_bytes = (size_t)PARTS * NT * KS * 256, red_bytes = (size_t)kStepWarps * R * P * 4;
-    static constexpr size_t smem = q_bytes + red_bytes + (size_t)kStepWarps * R * 8 + R * 4 + 64;
+template <int CODE, int P, int NT, int PARTS> struct step_sizes {
+    static constexpr int R = 8 * NT, KS = P / 16; // blocks of 16 value coordinates
     static constexpr int min_ctas = (P <= 128 && NT == 1) || (P == 64 && NT == 2) ? 2 : 1;
+    // queries: int8 digits for steps of 32 numbers, or fp16 parts for steps of 16
+    static constexpr bool digits = CODE == GGB_KV8_INT8;
+    static constexpr int Q = digits ? PARTS + 2 : PARTS, QS = digits ? P / 32 : P / 16;
+    static constexpr int half = 16 * P, stage = 2 * half; // a warp's 16 keys, then their values; S of them on their way or in use
+    static constexpr int S = P == 256 ? 3 : P == 128 ? (NT == 1 ? 3 : 6) : min_ctas == 2 ? 6 : 8;
+    static constexpr size_t q_bytes = (size_t)Q * NT * QS * 256, ring_bytes = (size_t)kStepWarps * S * stage, red_bytes = (size_t)kStepWarps * R * P * 4;
+    static_assert(red_bytes <= ring_bytes && stage % 1024 == 0, "the warps' sums lie over the stages");
+    static constexpr size_t smem = 1024 + q_bytes + ring_bytes + (size_t)kStepWarps * (R * 8 + 768) + R * 8 + 64;
+    static_assert((smem + 2048) * min_ctas <= 227 * 1024, "shared memory of an SM");
 };
 // where the pair of coordinates 2 i, 2 i + 1 of the 16 (P = 64: 8) numbers of lane group g lies in its row of the reduction, in pairs: rows of a warp's stores in different banks
 template <int P> __device__ __forceinline__ int red_at(int g, int i, int c) {
@@ -78,28 +114,97 @@ template <int P> __device__ __forceinline__ int red_at(int g, int i, int c) {
     return W * g + (i ^ ((((g >> 1) & 1) | (c << 1)) & (W - 1)));
 }
 
+// a row of queries to shared memory, by a warp: fp16 parts or int8 digits in the order of the lanes' pieces of a key, and what turns a product into a score (NaN where a query
+// is not finite: the row's own matter)
+template <int CODE, int P, int NT, int PARTS> __device__ __forceinline__ void stage_row(const attn_args &a, const float *src, bool real, int r, uint2 *sq, float *srow) {
+    using Z = step_sizes<CODE, P, NT, PARTS>;
+    const int lane = threadIdx.x & 31;
+    float4 x[(P + 127) / 128];
+    float m = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int k = 0; k < (P + 127) / 128; k++) {
+        const int d = 4 * lane + 128 * k;
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (real && d < a.D) {
+            if (a.vec_q) x[k] = *reinterpret_cast<const float4 *>(src + d);
+            else x[k] = make_float4(src[d], src[d + 1], src[d + 2], src[d + 3]);
+        }
+        const float t = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+        m = fmaxf(m, t);
+        odd |= t == INFINITY || x[k].x != x[k].x || x[k].y != x[k].y || x[k].z != x[k].z || x[k].w != x[k].w;
+    }
+    m = warp_max_f32(m);
+    odd = __any_sync(0xffffffffu, odd);
+    const float f = power_for(odd ? 0.f : m, Z::digits ? 7 * Z::Q - 2 : 10); // digits: the largest number below 2^(7 Q - 1), its first digit up to 64
+    if (lane == 0) srow[r] = odd ? NAN : (a.cap > 0.f ? 1.f : kLog2e) / f;
+#pragma unroll
+    for (int k = 0; k < (P + 127) / 128; k++) {
+        const int d = 4 * lane + 128 * k;
+        if (d >= P) break;
+        const float y[4] = {x[k].x * f, x[k].y * f, x[k].z * f, x[k].w * f};
+        const int t = r / 8, to = (r % 8) * 4 + (d % 64) / 16;
+        if (Z::digits) {
+            int n[4];
+            uint32_t *words = reinterpret_cast<uint32_t *>(sq + (t * Z::QS + 2 * (d / 64) + (d % 16) / 8) * 32 + to) + ((d >> 2) & 1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) n[e] = odd ? 0 : __float2int_rn(y[e]);
+#pragma unroll
+            for (int part = 0; part < Z::Q; part++) { // the last digit first
+                uint32_t word = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int digit = part == Z::Q - 1 ? n[e] : ((n[e] + 64) & 127) - 64;
+                    word |= (uint32_t)(digit & 255) << (8 * e);
+                    n[e] = (n[e] - digit) >> 7;
+                }
+                words[part * NT * Z::QS * 64] = word;
+            }
+        } else {
+            uint2 p = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
+            const int step = 4 * (d / 64) + (d % 16) / 4;
+            sq[(t * Z::QS + step) * 32 + to] = p;
+            if (PARTS == 2) {
+                const float2 b0 = half2_floats(p.x), b1 = half2_floats(p.y);
+                p = make_uint2(half2_bits(y[0] - b0.x, y[1] - b0.y), half2_bits(y[2] - b1.x, y[3] - b1.y));
+                sq[((NT + t) * Z::QS + step) * 32 + to] = p;
+            }
+        }
+    }
+}
+
 template <int CODE, int P, int NT, int PARTS>
-__global__ void __launch_bounds__(kStepThreads, step_sizes<P, NT, PARTS>::min_ctas) kv8_step_kernel(const __grid_constant__ attn_args a) {
-    using Z = step_sizes<P, NT, PARTS>;
+__global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::min_ctas) kv8_step_kernel(const __grid_constant__ attn_args a, const __grid_constant__ line_maps maps) {
+    using Z = step_sizes<CODE, P, NT, PARTS>;
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
     constexpr int R = Z::R, KS = Z::KS, NB = P / 64, VW = P == 64 ? 2 : 4, VC = P == 256 ? 2 : 1; // words of a lane's piece of a value row, pieces
     extern __shared__ __align__(16) uint8_t ks_smem[];
-    __shared__ int64_t s_scan[kStepWarps], s_at[2];
-    __shared__ int s_entry;
+    __shared__ int64_t s_scan[kStepWarps], s_u, s_end, s_all;
+    __shared__ int s_dead, s_entry, s_head, s_tile;
+    __shared__ item s_it;
+    __shared__ __align__(8) uint64_t s_bars[kStepWarps * Z::S];
     step_wait();
-    uint2 *sq = reinterpret_cast<uint2 *>(ks_smem);
-    float2 *red = reinterpret_cast<float2 *>(ks_smem + Z::q_bytes);
-    float *sm = reinterpret_cast<float *>(ks_smem + Z::q_bytes + Z::red_bytes), *sl = sm + kStepWarps * R, *srow = sl + kStepWarps * R, *svref = srow + R;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c4 = lane & 3, hpg = a.H / a.G;
+    volatile int *dead = &s_dead;
+    const uint32_t raw = smem_u32(ks_smem), ring0 = (raw + 1023u) & ~1023u;
+    uint8_t *base_at = ks_smem + (ring0 - raw);
+    float2 *red = reinterpret_cast<float2 *>(base_at); // over the stages
+    uint2 *sq = reinterpret_cast<uint2 *>(base_at + Z::ring_bytes);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c4 = lane & 3;
+    int2 *lines = reinterpret_cast<int2 *>(base_at + Z::ring_bytes + Z::q_bytes) + warp * 96; // [32]: lines of the tiles' keys and values
+    float2 *scales = reinterpret_cast<float2 *>(lines + 32);                                  // [64]
+    float *sm = reinterpret_cast<float *>(base_at + Z::ring_bytes + Z::q_bytes + kStepWarps * 768), *sl = sm + kStepWarps * R, *srow = sl + kStepWarps * R;
+    int *spos = reinterpret_cast<int *>(srow + R);
+    float *svref = reinterpret_cast<float *>(spos + R);
+    const uint32_t ring = ring0 + warp * Z::S * Z::stage, bars = smem_u32(s_bars) + 8 * warp * Z::S;
+    if (lane == 0)
+        for (int k = 0; k < Z::S; k++) mbar_init(bars + 8 * k, 1);
+    if (tid == 0) s_dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 
-    // ---- what this CTA has been dealt: units [u, u_end) of the tiles of all items, and where the first lies
-    int64_t u, u_end, U = 0;
-    int entry, head, tile;
-    item it;
-    const int entries = a.n_seq * a.groups;
+    // ---- what this CTA has been dealt: units [u, end) of the tiles of all items, and where the first lies
     if (a.part) {
-        const int each = (entries + kStepThreads - 1) / kStepThreads, e0 = min(entries, tid * each), e1 = min(entries, e0 + each);
-        int64_t mine = 0;
+        const int entries = a.n_seq * a.groups, each = (entries + kStepThreads - 1) / kStepThreads, e0 = min(entries, tid * each), e1 = min(entries, e0 + each);
+        int64_t mine = 0, U = 0, base = 0;
         for (int e = e0; e < e1; e++) mine += (int64_t)item_of<R>(a, e / a.groups, e % a.groups).n * a.G;
         int64_t run = mine;
 #pragma unroll
@@ -109,7 +214,6 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<P, NT, PARTS>::min_ct
         }
         if (lane == 31) s_scan[warp] = run;
         __syncthreads();
-        int64_t base = 0;
 #pragma unroll
         for (int w = 0; w < kStepWarps; w++) {
             if (w < warp) base += s_scan[w];
@@ -118,76 +222,90 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<P, NT, PARTS>::min_ct
         const int64_t N = min((int64_t)gridDim.x, U), b = blockIdx.x;
         if (tid == 0) a.desc[b] = make_int4(-1, 0, 0, 0);
         if (b >= N) return;
-        u = U * b / N, u_end = U * (b + 1) / N;
+        const int64_t u = U * b / N;
         base += run - mine;
         if (u >= base && u < base + mine) {
             int e = e0;
+            item it;
             for (;; e++) {
-                const int64_t n = (int64_t)item_of<R>(a, e / a.groups, e % a.groups).n * a.G;
-                if (u < base + n) break;
-                base += n;
+                it = item_of<R>(a, e / a.groups, e % a.groups);
+                if (u < base + (int64_t)it.n * a.G) break;
+                base += (int64_t)it.n * a.G;
             }
-            s_entry = e, s_at[0] = u - base;
+            s_it = it, s_entry = e, s_head = (int)((u - base) / it.n), s_tile = (int)((u - base) % it.n);
+            s_u = u, s_end = U * (b + 1) / N, s_all = U;
         }
-        __syncthreads();
-        entry = s_entry;
-        it = item_of<R>(a, entry / a.groups, entry % a.groups);
-        head = (int)(s_at[0] / it.n), tile = (int)(s_at[0] - (int64_t)head * it.n);
-    } else {
-        entry = blockIdx.x / a.G, head = blockIdx.x - entry * a.G, tile = 0;
-        it = item_of<R>(a, entry / a.groups, entry % a.groups);
-        u = 0, u_end = it.n;
+    } else if (tid == 0) {
+        s_entry = blockIdx.x / a.G, s_head = blockIdx.x - s_entry * a.G, s_tile = 0;
+        s_it = item_of<R>(a, s_entry / a.groups, s_entry % a.groups);
+        s_u = 0, s_end = s_it.n, s_all = 0;
     }
+    __syncthreads();
 
-    while (u < u_end) {
-        // ---- a piece of an item: tiles [tile, tile + n)
-        const int n = (int)min((int64_t)(it.n - tile), u_end - u);
-        // queries: rows as fp16 parts, in the order of a lane's pieces
+    int stage = 0; // stages are asked for and used in turn
+    uint32_t parity = 0;
+    while (s_u < s_end) {
+        // ---- a piece of an item: its tiles [tile, tile + n)
+        const int hpg = a.H / a.G, head = s_head, tile = s_tile, n = (int)min((int64_t)(s_it.n - tile), s_end - s_u);
         for (int r = warp; r < R; r += kStepWarps) {
-            float4 x[(P + 127) / 128];
-            float m = 0.f;
-            const int row = it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
-            const float *src = a.q + ((it.t0 + tq) * a.H + h) * a.D;
-#pragma unroll
-            for (int k = 0; k < (P + 127) / 128; k++) {
-                const int d = 4 * lane + 128 * k;
-                x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < it.rows && d < a.D) {
-                    if (a.vec_q) x[k] = *reinterpret_cast<const float4 *>(src + d);
-                    else x[k] = make_float4(src[d], src[d + 1], src[d + 2], src[d + 3]);
-                }
-                m = fmaxf(m, fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))));
-            }
-            m = warp_max_f32(m);
-            const float f = to_half_range(m);
-            if (lane == 0) srow[r] = (a.cap > 0.f ? 1.f : kLog2e) / f;
-            const float nan = m == INFINITY ? NAN : 0.f; // an infinite number spoils its row
-#pragma unroll
-            for (int k = 0; k < (P + 127) / 128; k++) {
-                const int d = 4 * lane + 128 * k;
-                if (d >= P) break;
-                const float y[4] = {x[k].x * f + nan, x[k].y * f + nan, x[k].z * f + nan, x[k].w * f + nan};
-                uint2 p = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
-                const int step = 4 * (d / 64) + (d % 16) / 4, to = (r % 8) * 4 + (d % 64) / 16;
-                sq[((r / 8) * KS + step) * 32 + to] = p;
-                if (PARTS == 2) {
-                    const float2 b0 = half2_floats(p.x), b1 = half2_floats(p.y);
-                    p = make_uint2(half2_bits(y[0] - b0.x, y[1] - b0.y), half2_bits(y[2] - b1.x, y[3] - b1.y));
-                    sq[((NT + r / 8) * KS + step) * 32 + to] = p;
-                }
-            }
+            const int row = s_it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
+            stage_row<CODE, P, NT, PARTS>(a, a.q + ((s_it.t0 + tq) * a.H + h) * a.D, r < s_it.rows, r, sq, srow);
+            if (lane == 0) spos[r] = r < s_it.rows ? s_it.p0 + tq : -1; // sees nothing
         }
+        fence_async_smem(); // sums that lay over the stages have been read
         __syncthreads();
-        float rowf[NT][2], m[NT][2], l[NT][2], o[KS][NT][4], vref = 0.f;
-        int pos[NT][2];
+
+        // the 16 positions of this warp in a tile.  32 tiles at a time, a lane each, are looked up: the lines of a group's keys (-1: no row sees any of it) and
+        // values, the scales of both (-1, too)
+        auto first_of = [&](int t) { return (t < s_it.kt ? t : s_it.w0 + t - s_it.kt) * kStepTile + 16 * warp; };
+        auto ask = [&](int k, int at_stage) {
+            if ((k & 31) == 0) {
+                const int t = tile + k + lane, first = first_of(t);
+                int2 line = make_int2(-1, 0);
+                float2 scale = make_float2(-1.f, 0.f);
+                if (k + lane < n && (t < s_it.kt ? first < s_it.n_keep : first + 15 >= s_it.lo && first <= s_it.i1)) {
+                    const int pg = first / a.B, grp = (first - pg * a.B) / kKv8Group;
+                    const int64_t rec = (int64_t)a.tables[s_it.s * a.table_ld + pg] * a.G + head;
+                    const float *sc = reinterpret_cast<const float *>(a.cache + rec * a.record + a.B * (a.D + a.Dv)) + grp;
+                    line.x = (int)(rec * (a.record / 128)) + grp * (a.D / 8);
+                    line.y = (int)(rec * (a.record / 128)) + a.B / kKv8Group * (a.D / 8) + grp * (a.Dv / 8);
+                    scale = make_float2(sc[0], sc[a.B / kKv8Group]);
+                }
+                scales[(k + lane) & 63] = scale, lines[lane] = line;
+                __syncwarp();
+            }
+            if (lane == 0) {
+                const int2 line = lines[k & 31];
+                const uint32_t to = ring + at_stage * Z::stage, bar = bars + 8 * at_stage;
+                if (line.x >= 0) request(maps, to, to + Z::half, line.x, line.y, 16 * (a.D + a.Dv), bar);
+                else mbar_arrive(bar);
+            }
+        };
+        // tiles [whole0, whole0 + wholes) of the window: every row sees all 16 positions
+        const int up = s_it.i0 - 15 - 16 * warp, down = max(s_it.lo, a.window > 0 ? (int)max((int64_t)0, s_it.i1 - a.window + 1) : 0) - 16 * warp;
+        const int whole0 = s_it.kt + max(0, (down + kStepTile - 1) / kStepTile - s_it.w0), wholes = up < 0 ? 0 : max(0, s_it.kt + up / kStepTile - s_it.w0 - whole0 + 1);
+
+        // where a lane's pieces lie in a stage (behind the end of a row: the row's first piece, which meets zeros of the queries or leaves by no coordinate)
+        uint32_t k_at[2][NB], v_at[4][VC];
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                k_at[e][b] = in_box((g8 + 8 * e) * a.D + (64 * b + 16 * c4 < a.D ? 64 * b + 16 * c4 : 0));
+                asm volatile("" : "+r"(k_at[e][b])); // computed once
+            }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int c = 0; c < VC; c++) {
+                v_at[e][c] = Z::half + in_box((2 * c4 + (e & 1) + 8 * (e >> 1)) * a.Dv + (128 * c + 4 * VW * g8 < a.Dv ? 128 * c + 4 * VW * g8 : 0));
+                asm volatile("" : "+r"(v_at[e][c]));
+            }
+        float rowf[NT][2], m[NT][2], l[NT][2], o[KS][NT][4], vref = 0.f, vinv = 0.f;
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int r = 8 * t + 2 * c4 + e;
-                rowf[t][e] = srow[r], m[t][e] = -INFINITY, l[t][e] = 0.f;
-                pos[t][e] = r < it.rows ? it.p0 + (it.row0 + r) / hpg : -1; // sees nothing
-            }
+            for (int e = 0; e < 2; e++) rowf[t][e] = srow[8 * t + 2 * c4 + e], m[t][e] = -INFINITY, l[t][e] = 0.f;
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
@@ -195,163 +313,181 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<P, NT, PARTS>::min_ct
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[i][t][e] = 0.f;
 
-        // the 16 positions of this warp in a tile: first one, or -1 where none of them is seen by any row
-        auto group_of = [&](int k) {
-            const int t = tile + k, first = (t < it.kt ? t : it.w0 + t - it.kt) * kStepTile + 16 * warp;
-            const int lo = t < it.kt ? 0 : it.lo, hi = t < it.kt ? it.n_keep - 1 : it.i1;
-            return k < n && first + 15 >= lo && first <= hi ? first : -1;
-        };
-        auto page_of = [&](int first) { return first < 0 ? 0 : a.tables[(int64_t)it.s * a.table_ld + first / a.B]; };
-        uint4 kx[2][NB];
-        uint32_t vx[4][VC][VW];
-        float ksc = 0.f, vsc = 0.f;
-        auto record_of = [&](int page) { return a.cache + ((int64_t)page * a.G + head) * a.record; };
-        auto load_k = [&](int first, int page) {
-            if (first < 0) return;
-            const int row = first % a.B, last = min(15, it.i1 - first); // rows behind the last position: the last one again
-            const uint8_t *rec = record_of(page);
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const uint8_t *k = rec + (int64_t)(row + min(g8 + 8 * e, last)) * a.D + 16 * c4;
-#pragma unroll
-                for (int b = 0; b < NB; b++) kx[e][b] = 64 * b + 16 * c4 < a.D ? ld_stream_u4(k + 64 * b) : make_uint4(0, 0, 0, 0);
-            }
-            const float *sc = reinterpret_cast<const float *>(rec + (int64_t)a.B * (a.D + a.Dv)) + row / kKv8Group;
-            ksc = sc[0], vsc = sc[a.B / kKv8Group];
-        };
-        auto load_v = [&](int first, int page) {
-            if (first < 0) return;
-            const int row = first % a.B, last = min(15, it.i1 - first);
-            const uint8_t *v0 = record_of(page) + (int64_t)a.B * a.D;
-#pragma unroll
-            for (int e = 0; e < 4; e++) { // keys 2 c4, 2 c4 + 1, 2 c4 + 8, 2 c4 + 9
-                const uint8_t *v = v0 + (int64_t)(row + min(2 * c4 + (e & 1) + 8 * (e >> 1), last)) * a.Dv + 4 * VW * g8;
-#pragma unroll
-                for (int c = 0; c < VC; c++) {
-                    if (VW == 4) {
-                        const uint4 x = 128 * c + 16 * g8 < a.Dv ? ld_stream_u4(v + 128 * c) : make_uint4(0, 0, 0, 0);
-                        vx[e][c][0] = x.x, vx[e][c][1] = x.y, vx[e][c][VW - 2] = x.z, vx[e][c][VW - 1] = x.w;
-                    } else {
-                        uint2 x = make_uint2(0, 0);
-                        if (8 * g8 < a.Dv) x = *reinterpret_cast<const uint2 *>(v);
-                        vx[e][c][0] = x.x, vx[e][c][1] = x.y;
-                    }
+        bool lost = *dead != 0; // a wait has run out: no more requests
+        parity ^= 1;            // (the first S turns only ask)
+        for (int k = -Z::S; k < n && !lost; k++) {
+            if (k >= 0) {
+                if (!mbar_wait_warp(bars + 8 * stage, parity, dead)) {
+                    lost = true;
+                    break;
                 }
-            }
-        };
-        int first = group_of(0), page = page_of(first);
-        load_k(first, page);
-        load_v(first, page);
-        int next = group_of(1), next_page = page_of(next);
-        for (int k = 0; k < n; k++) {
-            const int after = group_of(k + 2), after_page = page_of(after);
-            if (first >= 0) {
-                float z[NT][4];
+                const float2 sc = scales[k & 63];
+                if (sc.x >= 0.f) {
+                    const uint32_t from = ring + stage * Z::stage;
+                    float z[NT][4];
+                    uint4 kw[2][NB];
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                    for (int b = 0; b < NB; b++) kw[0][b] = lds_u4(from + k_at[0][b]), kw[1][b] = lds_u4(from + k_at[1][b]);
+                    if (Z::digits) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) z[t][e] = 0.f;
+                        for (int t = 0; t < NT; t++) {
+                            int zi[Z::Q][4];
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const uint32_t w0[4] = {kx[0][b].x, kx[0][b].y, kx[0][b].z, kx[0][b].w}, w1[4] = {kx[1][b].x, kx[1][b].y, kx[1][b].z, kx[1][b].w};
+                            for (int part = 0; part < Z::Q; part++)
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        uint32_t a0, a1, a2, a3;
-                        halves_of<CODE>(w0[w], a0, a2);
-                        halves_of<CODE>(w1[w], a1, a3);
+                                for (int e = 0; e < 4; e++) zi[part][e] = 0;
 #pragma unroll
-                        for (int part = PARTS - 1; part >= 0; part--)
+                            for (int b = 0; b < NB; b++)
 #pragma unroll
-                            for (int t = 0; t < NT; t++) {
-                                const uint2 y = sq[((part * NT + t) * KS + 4 * b + w) * 32 + lane];
-                                mma16816(z[t], a0, a1, a2, a3, y.x, y.y);
-                            }
-                    }
-                }
-                const float kscale = ksc, vscale = vsc;
-                load_k(next, next_page);
-                // ---- weights
-                const bool window_tile = tile + k >= it.kt;
-                const bool whole = first + 15 <= it.i0 && (window_tile ? first >= it.lo && (a.window <= 0 || first > it.i1 - a.window) : first + 15 < it.n_keep);
-                bool grow = false;
+                                for (int part = 0; part < Z::Q; part++) {
+                                    const uint2 y = sq[((part * NT + t) * Z::QS + 2 * b) * 32 + lane], x = sq[((part * NT + t) * Z::QS + 2 * b + 1) * 32 + lane];
+                                    mma16832(zi[part], kw[0][b].x, kw[1][b].x, kw[0][b].y, kw[1][b].y, y.x, y.y);
+                                    mma16832(zi[part], kw[0][b].z, kw[1][b].z, kw[0][b].w, kw[1][b].w, x.x, x.y);
+                                }
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float s = z[t][e] * (rowf[t][e & 1] * kscale);
-                        if (a.cap > 0.f) s = a.cap * kLog2e * tanhf(s / a.cap);
-                        if (!whole) {
-                            const int j = first + g8 + 8 * (e >> 1), i = pos[t][e & 1];
-                            const bool in_tile = window_tile ? j >= it.lo : j < it.n_keep;
-                            if (!(in_tile && j <= i && (a.window <= 0 || i - j < a.window || j < a.keep))) s = -INFINITY;
+                            for (int e = 0; e < 4; e++) // whole numbers below 2^29 each
+                                z[t][e] = Z::Q == 3 ? fmaf((float)(zi[2][e] * 128 + zi[1][e]), 128.f, (float)zi[0][e])
+                                                    : fmaf((float)(zi[Z::Q - 1][e] * 128 + zi[Z::Q - 2][e]), 16384.f, (float)(zi[1][e] * 128 + zi[0][e]));
                         }
-                        z[t][e] = s;
-                        grow |= s > m[t][e & 1] + 8.f;
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) z[t][e] = 0.f;
+#pragma unroll
+                        for (int b = 0; b < NB; b++) {
+                            const uint32_t w0[4] = {kw[0][b].x, kw[0][b].y, kw[0][b].z, kw[0][b].w}, w1[4] = {kw[1][b].x, kw[1][b].y, kw[1][b].z, kw[1][b].w};
+#pragma unroll
+                            for (int w = 0; w < 4; w++) {
+                                uint32_t a0, a1, a2, a3;
+                                halves_of<CODE>(w0[w], a0, a2);
+                                halves_of<CODE>(w1[w], a1, a3);
+#pragma unroll
+                                for (int part = PARTS - 1; part >= 0; part--)
+#pragma unroll
+                                    for (int t = 0; t < NT; t++) {
+                                        const uint2 y = sq[((part * NT + t) * Z::QS + 4 * b + w) * 32 + lane];
+                                        mma16816(z[t], a0, a1, a2, a3, y.x, y.y);
+                                    }
+                            }
+                        }
                     }
-                }
-                if (__any_sync(0xffffffffu, grow || vscale > 64.f * vref)) {
-                    const float vnew = vscale > 64.f * vref ? vscale : vref, vf = vnew > 0.f ? vref / vnew : 0.f;
-                    vref = vnew;
+                    // ---- weights
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float x = fmaxf(z[t][e], z[t][e + 2]);
+                        for (int e = 0; e < 4; e++) z[t][e] *= rowf[t][e & 1] * sc.x;
+                    if (a.cap > 0.f) {
 #pragma unroll
-                            for (int off = 4; off <= 16; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                            x = fmaxf(x, m[t][e]);
-                            const float f = m[t][e] == -INFINITY ? 0.f : exp2f(m[t][e] - x);
-                            m[t][e] = x;
-                            l[t][e] *= f;
+                        for (int t = 0; t < NT; t++)
 #pragma unroll
-                            for (int i = 0; i < KS; i++) o[i][t][e] *= f * vf, o[i][t][e + 2] *= f * vf;
-                        }
-                }
-                const float vrel = vref > 0.f ? vscale / vref : 0.f;
-                uint32_t pb[PARTS][NT][2];
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        w[e] = ex2_approx(z[t][e] - (m[t][e & 1] == -INFINITY ? 0.f : m[t][e & 1]));
-                        l[t][e & 1] += w[e];
-                        w[e] *= vrel;
+                            for (int e = 0; e < 4; e++) z[t][e] = a.cap * kLog2e * tanhf(z[t][e] / a.cap);
                     }
+                    if ((unsigned)(tile + k - whole0) >= (unsigned)wholes) {
+                        const int now = tile + k, first = first_of(now), i1 = s_it.i1;
+                        const int lo = now < s_it.kt ? 0 : s_it.lo, hi = now < s_it.kt ? s_it.n_keep - 1 : i1;
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        const uint32_t hi = half2_bits(w[2 * y], w[2 * y + 1]);
-                        pb[0][t][y] = turn8x8(hi);
-                        if (PARTS == 2) {
-                            const float2 back = half2_floats(hi);
-                            pb[PARTS - 1][t][y] = turn8x8(half2_bits(w[2 * y] - back.x, w[2 * y + 1] - back.y));
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int j = first + g8 + 8 * (e >> 1), i = spos[8 * t + 2 * c4 + (e & 1)];
+                                if (!(j >= lo && j <= hi && j <= i && (a.window <= 0 || i - j < a.window || j < a.keep))) z[t][e] = -INFINITY;
+                            }
+                        // behind the last position there may be e4m3 codes that are no numbers, whose weight of zero would spoil a sum
+                        if (CODE == GGB_KV8_E4M3 && first + 15 > i1) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (first + 2 * c4 + (e & 1) + 8 * (e >> 1) > i1)
+#pragma unroll
+                                    for (int c = 0; c < VC; c++) {
+                                        asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c]), "r"(0u) : "memory");
+                                        if (VW == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c] + 8), "r"(0u) : "memory");
+                                    }
+                            fence_async_smem();
+                            __syncwarp();
                         }
                     }
-                }
-                // ---- output: coordinates 2 i, 2 i + 1 of a lane's piece are rows g8 and g8 + 8 of block i
+                    bool grow = sc.y > 64.f * vref;
 #pragma unroll
-                for (int c = 0; c < VC; c++)
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int w = 0; w < VW; w++)
+                        for (int e = 0; e < 4; e++) grow |= z[t][e] > m[t][e & 1] + 8.f;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float vnew = sc.y > 64.f * vref ? sc.y : vref, vf = vnew > 0.f ? vref / vnew : 0.f;
+                        vref = vnew, vinv = vnew > 0.f ? 1.f / vnew : 0.f;
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                float x = fmaxf(z[t][e], z[t][e + 2]);
+#pragma unroll
+                                for (int off = 4; off <= 16; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+                                x = fmaxf(x, m[t][e]);
+                                const float f = m[t][e] == -INFINITY ? 0.f : exp2f(m[t][e] - x);
+                                m[t][e] = x;
+                                l[t][e] *= f;
+#pragma unroll
+                                for (int i = 0; i < KS; i++) o[i][t][e] *= f * vf, o[i][t][e + 2] *= f * vf;
+                            }
+                    }
+                    const float vrel = sc.y * vinv;
+                    uint32_t pb[PARTS][NT][2];
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            w[e] = ex2_approx(z[t][e] - (m[t][e & 1] == -INFINITY ? 0.f : m[t][e & 1]));
+                            l[t][e & 1] += w[e];
+                            w[e] *= vrel;
+                        }
 #pragma unroll
                         for (int y = 0; y < 2; y++) {
-                            const uint32_t sel = y ? 0x7362 : 0x5140;
-                            uint32_t a0, a1, a2, a3;
-                            halves_of<CODE>(__byte_perm(vx[0][c][w], vx[1][c][w], sel), a0, a1);
-                            halves_of<CODE>(__byte_perm(vx[2][c][w], vx[3][c][w], sel), a2, a3);
-#pragma unroll
-                            for (int part = PARTS - 1; part >= 0; part--)
-#pragma unroll
-                                for (int t = 0; t < NT; t++) mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[part][t][0], pb[part][t][1]);
+                            const uint32_t hi = half2_bits(w[2 * y], w[2 * y + 1]);
+                            pb[0][t][y] = turn8x8(hi);
+                            if (PARTS == 2) {
+                                const float2 back = half2_floats(hi);
+                                pb[PARTS - 1][t][y] = turn8x8(half2_bits(w[2 * y] - back.x, w[2 * y + 1] - back.y));
+                            }
                         }
-            } else {
-                load_k(next, next_page);
+                    }
+                    // ---- output: coordinates 2 i, 2 i + 1 of a lane's piece are rows g8 and g8 + 8 of block i
+#pragma unroll
+                    for (int c = 0; c < VC; c++) {
+                        uint32_t vx[4][VW];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (VW == 4) {
+                                const uint4 x = lds_u4(from + v_at[e][c]);
+                                vx[e][0] = x.x, vx[e][1] = x.y, vx[e][VW - 2] = x.z, vx[e][VW - 1] = x.w;
+                            } else {
+                                const uint2 x = lds_u2(from + v_at[e][c]);
+                                vx[e][0] = x.x, vx[e][1] = x.y;
+                            }
+                        }
+#pragma unroll
+                        for (int w = 0; w < VW; w++)
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                const uint32_t sel = y ? 0x7362 : 0x5140;
+                                uint32_t a0, a1, a2, a3;
+                                halves_of<CODE>(__byte_perm(vx[0][w], vx[1][w], sel), a0, a1);
+                                halves_of<CODE>(__byte_perm(vx[2][w], vx[3][w], sel), a2, a3);
+#pragma unroll
+                                for (int part = PARTS - 1; part >= 0; part--)
+#pragma unroll
+                                    for (int t = 0; t < NT; t++) mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[part][t][0], pb[part][t][1]);
+                            }
+                    }
+                }
+                __syncwarp();
             }
-            load_v(next, next_page);
-            first = next, page = next_page, next = after, next_page = after_page;
+            if (k + Z::S < n) ask(k + Z::S, stage); // what has been used
+            if (++stage == Z::S) stage = 0, parity ^= 1;
         }
 
         // ---- the warps' sums meet
+        __syncthreads(); // (every group that was asked for has been used)
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -366,11 +502,11 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<P, NT, PARTS>::min_ct
             }
         if (lane == 0) svref[warp] = vref;
         __syncthreads();
-        const bool whole_item = n == it.n;
+        const bool whole_item = n == s_it.n;
         float *part = a.part ? a.part + ((int64_t)blockIdx.x * 2 + (tile == 0)) * R * (a.Dv + 2) : nullptr;
         constexpr int TPR = kStepThreads / R; // threads a row
         const int r = tid / TPR;
-        if (r < it.rows) {
+        if (r < s_it.rows) {
             float M = -INFINITY, L = 0.f, f[kStepWarps];
 #pragma unroll
             for (int w = 0; w < kStepWarps; w++) M = fmaxf(M, sm[w * R + r]);
@@ -380,8 +516,8 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<P, NT, PARTS>::min_ct
                 L = fmaf(sl[w * R + r], f[w], L);
                 f[w] *= svref[w];
             }
-            const int row = it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
-            const int64_t t = it.t0 + tq;
+            const int row = s_it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
+            const int64_t t = s_it.t0 + tq;
             const row_end end(a, h, M, L);
             for (int pr = tid - r * TPR; pr < a.Dv / 2; pr += TPR) {
                 constexpr int W = P == 64 ? 4 : 8;
@@ -403,20 +539,25 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<P, NT, PARTS>::min_ct
             if (!whole_item && tid == r * TPR) part[(int64_t)r * (a.Dv + 2) + a.Dv] = M, part[(int64_t)r * (a.Dv + 2) + a.Dv + 1] = L;
         }
         if (!whole_item && tile == 0 && tid == 0) { // it ends with the CTA that has its last tile
-            const int64_t N = min((int64_t)gridDim.x, U), last = u - tile + it.n - 1;
-            a.desc[blockIdx.x] = make_int4(it.s, it.rg, head, (int)(((last + 1) * N - 1) / U));
+            const int64_t N = min((int64_t)gridDim.x, s_all), last = s_u - tile + s_it.n - 1;
+            a.desc[blockIdx.x] = make_int4(s_it.s, s_it.rg, head, (int)(((last + 1) * N - 1) / s_all));
         }
-        u += n;
-        if (u >= u_end) break;
         __syncthreads(); // what is read above is written by the next piece
-        tile = 0;
-        if (++head == a.G) {
-            head = 0;
-            do {
-                entry++;
-                it = item_of<R>(a, entry / a.groups, entry % a.groups);
-            } while (it.n == 0);
+        if (tid == 0) {
+            s_u += n, s_tile = 0;
+            if (s_u < s_end && ++s_head == a.G) {
+                s_head = 0;
+                do {
+                    s_entry++;
+                    s_it = item_of<R>(a, s_entry / a.groups, s_entry % a.groups);
+                } while (s_it.n == 0);
+            }
         }
+        __syncthreads();
+    }
+    if (warp == 0) {
+        settle(dead);
+        if (lane == 0 && *dead) *a.wait_error = 1;
     }
 }
 
@@ -477,16 +618,20 @@ template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_ker
 }
 
 template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64_t max_new) {
-    using Z = step_sizes<P, NT, PARTS>;
+    using Z = step_sizes<CODE, P, NT, PARTS>;
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
     const int64_t groups = (max_new * (a.H / a.G) + Z::R - 1) / Z::R;
     GGB_CHECK_ARG(max_new * (a.H / a.G) < (1ll << 30) && a.n_seq * groups * a.G < (1ll << 31), "kv8_attn: too many sequences, tokens and heads for a launch");
     a.groups = (int)groups;
     auto k = kv8_step_kernel<CODE, P, NT, PARTS>;
-    const int rc = ggb_allow_smem(k, Z::smem);
+    int rc = ggb_allow_smem(k, Z::smem);
     if (rc) return rc;
     const unsigned ctas = a.part ? (unsigned)std::min(kMaxCtas, ggb_sm_count() * Z::min_ctas) : (unsigned)(a.n_seq * a.groups * a.G);
-    GGB_CUDA(ggb_launch_step(k, dim3(ctas), dim3(kStepThreads), Z::smem, a));
+    line_maps maps;
+    rc = ggb_tensor_map_bf16(&maps.k, a.cache, (1ll << 31) - 1, 64, 64, a.D / 8);
+    if (!rc) rc = ggb_tensor_map_bf16(&maps.v, a.cache, (1ll << 31) - 1, 64, 64, a.Dv / 8);
+    if (rc) return rc;
+    GGB_CUDA(ggb_launch_step(k, dim3(ctas), dim3(kStepThreads), Z::smem, a, maps));
     GGB_LAUNCH_CHECK();
     if (a.part) {
         GGB_CUDA(ggb_launch_step(kv8_join_kernel<Z::R, E>, dim3(ctas, Z::R), dim3(256), 0, a));
@@ -528,7 +673,7 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
     float *part = (float *)scratch;
     const attn_args a{q, (const uint8_t *)cache, tables, table_ld, block_size, n_seq, starts, pos0, H, G, D, Dv, window, window > 0 ? keep_first : 0, softcap, sink, gate, ldg,
                            kv8_record(D, Dv, block_size), out, 0, part, part ? (int4 *)(part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2)) : nullptr,
-                           (uintptr_t)q % 16 == 0};
+                           (uintptr_t)q % 16 == 0, ggb_wait_error_flag()};
     if (dt == GGB_TYPE_BF16) return code == GGB_KV8_INT8 ? step_rows<GGB_KV8_INT8, 1>(a, max_new) : step_rows<GGB_KV8_E4M3, 1>(a, max_new);
     return code == GGB_KV8_INT8 ? step_rows<GGB_KV8_INT8, 2>(a, max_new) : step_rows<GGB_KV8_E4M3, 2>(a, max_new);
 }
