@@ -31,6 +31,7 @@ using namespace kv8;
 
 constexpr int kStepWarps = 8, kStepThreads = 32 * kStepWarps, kStepTile = 16 * kStepWarps; // keys of a tile
 constexpr int kMaxRows = 32, kMaxCtas = 512;
+constexpr float kNone = -3e38f; // a maximum of nothing: a number, so that the differences to it are
 
 inline size_t part_bytes(int Dv) { return (size_t)kMaxCtas * (2 * kMaxRows * (size_t)(Dv + 2) * 4 + sizeof(int4)); }
 
@@ -61,6 +62,17 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same on sums that begin with it
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma16832_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -247,14 +259,6 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
     while (s_u < s_end) {
         // ---- a piece of an item: its tiles [tile, tile + n)
         const int hpg = a.H / a.G, head = s_head, tile = s_tile, n = (int)min((int64_t)(s_it.n - tile), s_end - s_u);
-        for (int r = warp; r < R; r += kStepWarps) {
-            const int row = s_it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
-            stage_row<CODE, P, NT, PARTS>(a, a.q + ((s_it.t0 + tq) * a.H + h) * a.D, r < s_it.rows, r, sq, srow);
-            if (lane == 0) spos[r] = r < s_it.rows ? s_it.p0 + tq : -1; // sees nothing
-        }
-        fence_async_smem(); // sums that lay over the stages have been read
-        __syncthreads();
-
         // the 16 positions of this warp in a tile.  32 tiles at a time, a lane each, are looked up: the lines of a group's keys (-1: no row sees any of it) and
         // values, the scales of both (-1, too)
         auto first_of = [&](int t) { return (t < s_it.kt ? t : s_it.w0 + t - s_it.kt) * kStepTile + 16 * warp; };
@@ -301,11 +305,22 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
                 v_at[e][c] = Z::half + in_box((2 * c4 + (e & 1) + 8 * (e >> 1)) * a.Dv + (128 * c + 4 * VW * g8 < a.Dv ? 128 * c + 4 * VW * g8 : 0));
                 asm volatile("" : "+r"(v_at[e][c]));
             }
+        bool lost = *dead != 0; // a wait has run out: no more requests
+        for (int k = 0, s = stage; k < Z::S && k < n && !lost; k++) {
+            ask(k, s);
+            if (++s == Z::S) s = 0;
+        }
+        for (int r = warp; r < R; r += kStepWarps) {
+            const int row = s_it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
+            stage_row<CODE, P, NT, PARTS>(a, a.q + ((s_it.t0 + tq) * a.H + h) * a.D, r < s_it.rows, r, sq, srow);
+            if (lane == 0) spos[r] = r < s_it.rows ? s_it.p0 + tq : -1; // sees nothing
+        }
+        __syncthreads();
         float rowf[NT][2], m[NT][2], l[NT][2], o[KS][NT][4], vref = 0.f, vinv = 0.f;
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) rowf[t][e] = srow[8 * t + 2 * c4 + e], m[t][e] = -INFINITY, l[t][e] = 0.f;
+            for (int e = 0; e < 2; e++) rowf[t][e] = srow[8 * t + 2 * c4 + e], m[t][e] = kNone, l[t][e] = 0.f;
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
@@ -313,175 +328,162 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[i][t][e] = 0.f;
 
-        bool lost = *dead != 0; // a wait has run out: no more requests
-        parity ^= 1;            // (the first S turns only ask)
-        for (int k = -Z::S; k < n && !lost; k++) {
-            if (k >= 0) {
-                if (!mbar_wait_warp(bars + 8 * stage, parity, dead)) {
-                    lost = true;
-                    break;
-                }
-                const float2 sc = scales[k & 63];
-                if (sc.x >= 0.f) {
-                    const uint32_t from = ring + stage * Z::stage;
-                    float z[NT][4];
-                    uint4 kw[2][NB];
+        for (int k = 0; k < n && !lost; k++) {
+            if (!mbar_wait_warp(bars + 8 * stage, parity, dead)) break;
+            const float2 sc = scales[k & 63];
+            if (sc.x >= 0.f) {
+                const uint32_t from = ring + stage * Z::stage;
+                float z[NT][4];
+                uint4 kw[2][NB];
 #pragma unroll
-                    for (int b = 0; b < NB; b++) kw[0][b] = lds_u4(from + k_at[0][b]), kw[1][b] = lds_u4(from + k_at[1][b]);
-                    if (Z::digits) {
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            int zi[Z::Q][4];
-#pragma unroll
-                            for (int part = 0; part < Z::Q; part++)
-#pragma unroll
-                                for (int e = 0; e < 4; e++) zi[part][e] = 0;
-#pragma unroll
-                            for (int b = 0; b < NB; b++)
-#pragma unroll
-                                for (int part = 0; part < Z::Q; part++) {
-                                    const uint2 y = sq[((part * NT + t) * Z::QS + 2 * b) * 32 + lane], x = sq[((part * NT + t) * Z::QS + 2 * b + 1) * 32 + lane];
-                                    mma16832(zi[part], kw[0][b].x, kw[1][b].x, kw[0][b].y, kw[1][b].y, y.x, y.y);
-                                    mma16832(zi[part], kw[0][b].z, kw[1][b].z, kw[0][b].w, kw[1][b].w, x.x, x.y);
-                                }
-#pragma unroll
-                            for (int e = 0; e < 4; e++) // whole numbers below 2^29 each
-                                z[t][e] = Z::Q == 3 ? fmaf((float)(zi[2][e] * 128 + zi[1][e]), 128.f, (float)zi[0][e])
-                                                    : fmaf((float)(zi[Z::Q - 1][e] * 128 + zi[Z::Q - 2][e]), 16384.f, (float)(zi[1][e] * 128 + zi[0][e]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) z[t][e] = 0.f;
-#pragma unroll
-                        for (int b = 0; b < NB; b++) {
-                            const uint32_t w0[4] = {kw[0][b].x, kw[0][b].y, kw[0][b].z, kw[0][b].w}, w1[4] = {kw[1][b].x, kw[1][b].y, kw[1][b].z, kw[1][b].w};
-#pragma unroll
-                            for (int w = 0; w < 4; w++) {
-                                uint32_t a0, a1, a2, a3;
-                                halves_of<CODE>(w0[w], a0, a2);
-                                halves_of<CODE>(w1[w], a1, a3);
-#pragma unroll
-                                for (int part = PARTS - 1; part >= 0; part--)
-#pragma unroll
-                                    for (int t = 0; t < NT; t++) {
-                                        const uint2 y = sq[((part * NT + t) * Z::QS + 4 * b + w) * 32 + lane];
-                                        mma16816(z[t], a0, a1, a2, a3, y.x, y.y);
-                                    }
-                            }
-                        }
-                    }
-                    // ---- weights
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) z[t][e] *= rowf[t][e & 1] * sc.x;
-                    if (a.cap > 0.f) {
-#pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) z[t][e] = a.cap * kLog2e * tanhf(z[t][e] / a.cap);
-                    }
-                    if ((unsigned)(tile + k - whole0) >= (unsigned)wholes) {
-                        const int now = tile + k, first = first_of(now), i1 = s_it.i1;
-                        const int lo = now < s_it.kt ? 0 : s_it.lo, hi = now < s_it.kt ? s_it.n_keep - 1 : i1;
-#pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int j = first + g8 + 8 * (e >> 1), i = spos[8 * t + 2 * c4 + (e & 1)];
-                                if (!(j >= lo && j <= hi && j <= i && (a.window <= 0 || i - j < a.window || j < a.keep))) z[t][e] = -INFINITY;
-                            }
-                        // behind the last position there may be e4m3 codes that are no numbers, whose weight of zero would spoil a sum
-                        if (CODE == GGB_KV8_E4M3 && first + 15 > i1) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (first + 2 * c4 + (e & 1) + 8 * (e >> 1) > i1)
-#pragma unroll
-                                    for (int c = 0; c < VC; c++) {
-                                        asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c]), "r"(0u) : "memory");
-                                        if (VW == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c] + 8), "r"(0u) : "memory");
-                                    }
-                            fence_async_smem();
-                            __syncwarp();
-                        }
-                    }
-                    bool grow = sc.y > 64.f * vref;
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) grow |= z[t][e] > m[t][e & 1] + 8.f;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float vnew = sc.y > 64.f * vref ? sc.y : vref, vf = vnew > 0.f ? vref / vnew : 0.f;
-                        vref = vnew, vinv = vnew > 0.f ? 1.f / vnew : 0.f;
-#pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                float x = fmaxf(z[t][e], z[t][e + 2]);
-#pragma unroll
-                                for (int off = 4; off <= 16; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                                x = fmaxf(x, m[t][e]);
-                                const float f = m[t][e] == -INFINITY ? 0.f : exp2f(m[t][e] - x);
-                                m[t][e] = x;
-                                l[t][e] *= f;
-#pragma unroll
-                                for (int i = 0; i < KS; i++) o[i][t][e] *= f * vf, o[i][t][e + 2] *= f * vf;
-                            }
-                    }
-                    const float vrel = sc.y * vinv;
-                    uint32_t pb[PARTS][NT][2];
+                for (int b = 0; b < NB; b++) kw[0][b] = lds_u4(from + k_at[0][b]), kw[1][b] = lds_u4(from + k_at[1][b]);
+                if (Z::digits) {
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        float w[4];
+                        int zi[Z::Q][4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            w[e] = ex2_approx(z[t][e] - (m[t][e & 1] == -INFINITY ? 0.f : m[t][e & 1]));
-                            l[t][e & 1] += w[e];
-                            w[e] *= vrel;
-                        }
+                        for (int b = 0; b < NB; b++)
 #pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            const uint32_t hi = half2_bits(w[2 * y], w[2 * y + 1]);
-                            pb[0][t][y] = turn8x8(hi);
-                            if (PARTS == 2) {
-                                const float2 back = half2_floats(hi);
-                                pb[PARTS - 1][t][y] = turn8x8(half2_bits(w[2 * y] - back.x, w[2 * y + 1] - back.y));
+                            for (int part = 0; part < Z::Q; part++) {
+                                const uint2 y = sq[((part * NT + t) * Z::QS + 2 * b) * 32 + lane], x = sq[((part * NT + t) * Z::QS + 2 * b + 1) * 32 + lane];
+                                if (b == 0) mma16832_first(zi[part], kw[0][b].x, kw[1][b].x, kw[0][b].y, kw[1][b].y, y.x, y.y);
+                                else mma16832(zi[part], kw[0][b].x, kw[1][b].x, kw[0][b].y, kw[1][b].y, y.x, y.y);
+                                mma16832(zi[part], kw[0][b].z, kw[1][b].z, kw[0][b].w, kw[1][b].w, x.x, x.y);
                             }
-                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) // whole numbers below 2^29 each
+                            z[t][e] = Z::Q == 3 ? fmaf((float)(zi[2][e] * 128 + zi[1][e]), 128.f, (float)zi[0][e])
+                                                : fmaf((float)(zi[Z::Q - 1][e] * 128 + zi[Z::Q - 2][e]), 16384.f, (float)(zi[1][e] * 128 + zi[0][e]));
                     }
-                    // ---- output: coordinates 2 i, 2 i + 1 of a lane's piece are rows g8 and g8 + 8 of block i
+                } else {
 #pragma unroll
-                    for (int c = 0; c < VC; c++) {
-                        uint32_t vx[4][VW];
+                    for (int b = 0; b < NB; b++) {
+                        const uint32_t w0[4] = {kw[0][b].x, kw[0][b].y, kw[0][b].z, kw[0][b].w}, w1[4] = {kw[1][b].x, kw[1][b].y, kw[1][b].z, kw[1][b].w};
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if (VW == 4) {
-                                const uint4 x = lds_u4(from + v_at[e][c]);
-                                vx[e][0] = x.x, vx[e][1] = x.y, vx[e][VW - 2] = x.z, vx[e][VW - 1] = x.w;
-                            } else {
-                                const uint2 x = lds_u2(from + v_at[e][c]);
-                                vx[e][0] = x.x, vx[e][1] = x.y;
-                            }
+                        for (int w = 0; w < 4; w++) {
+                            uint32_t a0, a1, a2, a3;
+                            halves_of<CODE>(w0[w], a0, a2);
+                            halves_of<CODE>(w1[w], a1, a3);
+#pragma unroll
+                            for (int part = PARTS - 1; part >= 0; part--)
+#pragma unroll
+                                for (int t = 0; t < NT; t++) {
+                                    const uint2 y = sq[((part * NT + t) * Z::QS + 4 * b + w) * 32 + lane];
+                                    if (b + w == 0 && part == PARTS - 1) mma16816_first(z[t], a0, a1, a2, a3, y.x, y.y);
+                                    else mma16816(z[t], a0, a1, a2, a3, y.x, y.y);
+                                }
                         }
-#pragma unroll
-                        for (int w = 0; w < VW; w++)
-#pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                const uint32_t sel = y ? 0x7362 : 0x5140;
-                                uint32_t a0, a1, a2, a3;
-                                halves_of<CODE>(__byte_perm(vx[0][w], vx[1][w], sel), a0, a1);
-                                halves_of<CODE>(__byte_perm(vx[2][w], vx[3][w], sel), a2, a3);
-#pragma unroll
-                                for (int part = PARTS - 1; part >= 0; part--)
-#pragma unroll
-                                    for (int t = 0; t < NT; t++) mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[part][t][0], pb[part][t][1]);
-                            }
                     }
                 }
-                __syncwarp();
+                // ---- weights
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z[t][e] *= rowf[t][e & 1] * sc.x;
+                if (a.cap > 0.f) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) z[t][e] = a.cap * kLog2e * tanhf(z[t][e] / a.cap);
+                }
+                if ((unsigned)(tile + k - whole0) >= (unsigned)wholes) {
+                    const int now = tile + k, first = first_of(now), i1 = s_it.i1;
+                    const int lo = now < s_it.kt ? 0 : s_it.lo, hi = now < s_it.kt ? s_it.n_keep - 1 : i1;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int j = first + g8 + 8 * (e >> 1), i = spos[8 * t + 2 * c4 + (e & 1)];
+                            if (!(j >= lo && j <= hi && j <= i && (a.window <= 0 || i - j < a.window || j < a.keep))) z[t][e] = -INFINITY;
+                        }
+                    // behind the last position there may be e4m3 codes that are no numbers, whose weight of zero would spoil a sum
+                    if (CODE == GGB_KV8_E4M3 && first + 15 > i1) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (first + 2 * c4 + (e & 1) + 8 * (e >> 1) > i1)
+#pragma unroll
+                                for (int c = 0; c < VC; c++) {
+                                    asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c]), "r"(0u) : "memory");
+                                    if (VW == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c] + 8), "r"(0u) : "memory");
+                                }
+                        fence_async_smem();
+                        __syncwarp();
+                    }
+                }
+                bool grow = sc.y > 64.f * vref;
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) grow |= z[t][e] > m[t][e & 1] + 8.f;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float vnew = sc.y > 64.f * vref ? sc.y : vref, vf = vnew > 0.f ? vref / vnew : 0.f;
+                    vref = vnew, vinv = vnew > 0.f ? 1.f / vnew : 0.f;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float x = fmaxf(z[t][e], z[t][e + 2]);
+#pragma unroll
+                            for (int off = 4; off <= 16; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+                            x = fmaxf(x, m[t][e]);
+                            const float f = exp2f(m[t][e] - x);
+                            m[t][e] = x;
+                            l[t][e] *= f;
+#pragma unroll
+                            for (int i = 0; i < KS; i++) o[i][t][e] *= f * vf, o[i][t][e + 2] *= f * vf;
+                        }
+                }
+                const float vrel = sc.y * vinv;
+                uint32_t pb[PARTS][NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        w[e] = ex2_approx(z[t][e] - m[t][e & 1]);
+                        l[t][e & 1] += w[e];
+                        w[e] *= vrel;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 2; y++) {
+                        const uint32_t hi = half2_bits(w[2 * y], w[2 * y + 1]);
+                        pb[0][t][y] = turn8x8(hi);
+                        if (PARTS == 2) {
+                            const float2 back = half2_floats(hi);
+                            pb[PARTS - 1][t][y] = turn8x8(half2_bits(w[2 * y] - back.x, w[2 * y + 1] - back.y));
+                        }
+                    }
+                }
+                // ---- output: coordinates 2 i, 2 i + 1 of a lane's piece are rows g8 and g8 + 8 of block i
+#pragma unroll
+                for (int c = 0; c < VC; c++) {
+                    uint32_t vx[4][VW];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (VW == 4) {
+                            const uint4 x = lds_u4(from + v_at[e][c]);
+                            vx[e][0] = x.x, vx[e][1] = x.y, vx[e][VW - 2] = x.z, vx[e][VW - 1] = x.w;
+                        } else {
+                            const uint2 x = lds_u2(from + v_at[e][c]);
+                            vx[e][0] = x.x, vx[e][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < VW; w++)
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const uint32_t sel = y ? 0x7362 : 0x5140;
+                            uint32_t a0, a1, a2, a3;
+                            halves_of<CODE>(__byte_perm(vx[0][w], vx[1][w], sel), a0, a1);
+                            halves_of<CODE>(__byte_perm(vx[2][w], vx[3][w], sel), a2, a3);
+#pragma unroll
+                            for (int part = PARTS - 1; part >= 0; part--)
+#pragma unroll
+                                for (int t = 0; t < NT; t++) mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[part][t][0], pb[part][t][1]);
+                        }
+                }
             }
+            __syncwarp();
             if (k + Z::S < n) ask(k + Z::S, stage); // what has been used
             if (++stage == Z::S) stage = 0, parity ^= 1;
         }
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
             for (int w = 0; w < kStepWarps; w++) M = fmaxf(M, sm[w * R + r]);
 #pragma unroll
             for (int w = 0; w < kStepWarps; w++) {
-                f[w] = sm[w * R + r] == -INFINITY ? 0.f : exp2f(sm[w * R + r] - M);
+                f[w] = exp2f(sm[w * R + r] - M);
                 L = fmaf(sl[w * R + r], f[w], L);
                 f[w] *= svref[w];
             }
@@ -542,7 +544,8 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
             const int64_t N = min((int64_t)gridDim.x, s_all), last = s_u - tile + s_it.n - 1;
             a.desc[blockIdx.x] = make_int4(s_it.s, s_it.rg, head, (int)(((last + 1) * N - 1) / s_all));
         }
-        __syncthreads(); // what is read above is written by the next piece
+        fence_async_smem();
+        __syncthreads(); // what is read above is written by the next piece, sums by its copies
         if (tid == 0) {
             s_u += n, s_tile = 0;
             if (s_u < s_end && ++s_head == a.G) {
@@ -583,7 +586,7 @@ template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_ker
     for (int w = 0; w < 8; w++) M = fmaxf(M, s_red[w]);
     float L = 0.f;
     for (int k = tid; k < pieces; k += 256) {
-        const float f = s_f[k] == -INFINITY ? 0.f : exp2f(s_f[k] - M);
+        const float f = exp2f(s_f[k] - M);
         L = fmaf(piece(k)[a.Dv + 1], f, L);
         s_f[k] = f;
     }
