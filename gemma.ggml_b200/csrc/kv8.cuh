@@ -67,7 +67,7 @@ struct attn_args {
     void *out;
     int groups;     // items of a sequence and key head, at most
     float *part;    // [CTA][2][rows][Dv + 2], or null: an item a CTA
-    int4 *desc;     // [CTA]: sequence (or -1), group of rows, key head, last CTA of the item that begins here and ends elsewhere
+    int4 *desc;     // [CTA][2], of an item that begins or goes on here and ends elsewhere: sequence (or -1), rows, key head, first row; first and last CTA that have it, first token
     int vec_q;      // queries begin on a 16-byte boundary
     int *wait_error;
 };

@@ -29,20 +29,19 @@ namespace {
 
 using namespace kv8;
 
-constexpr int kStepWarps = 8, kStepThreads = 32 * kStepWarps, kStepTile = 16 * kStepWarps; // keys of a tile
 constexpr int kMaxRows = 32, kMaxCtas = 512;
 constexpr float kNone = -3e38f; // a maximum of nothing: a number, so that the differences to it are
 
-inline size_t part_bytes(int Dv) { return (size_t)kMaxCtas * (2 * kMaxRows * (size_t)(Dv + 2) * 4 + sizeof(int4)); }
+inline size_t part_bytes(int Dv) { return (size_t)kMaxCtas * (2 * kMaxRows * (size_t)(Dv + 2) * 4 + 2 * sizeof(int4)); }
 
-// the rows of an item and the tiles that they see: [0, n_keep) in kt tiles, then [lo, i1] in tiles from position kStepTile * w0 on
+// the rows of an item and the tiles that they see: [0, n_keep) in kt tiles, then [lo, i1] in tiles from position TILE * w0 on
 struct item {
     int s, rg, row0, rows; // rows [row0, row0 + rows) of the sequence: its tokens x the query heads of a key head
     int p0, i0, i1;        // positions of its first token, of the item's first and last
     int lo, n_keep, kt, w0, n;
     int64_t t0;            // its first token
 };
-template <int R> __device__ __forceinline__ item item_of(const attn_args &a, int s, int rg) {
+template <int R, int TILE> __device__ __forceinline__ item item_of(const attn_args &a, int s, int rg) {
     item x;
     const int hpg = a.H / a.G;
     x.s = s, x.rg = rg, x.t0 = a.starts[s], x.p0 = a.pos0[s], x.row0 = rg * R;
@@ -53,9 +52,41 @@ template <int R> __device__ __forceinline__ item item_of(const attn_args &a, int
     x.i0 = x.p0 + x.row0 / hpg, x.i1 = x.p0 + (x.row0 + x.rows - 1) / hpg;
     x.lo = a.window > 0 ? (int)max((int64_t)0, x.i0 - a.window + 1) : 0;
     x.n_keep = (int)min(a.keep, (int64_t)x.lo);
-    x.kt = (x.n_keep + kStepTile - 1) / kStepTile, x.w0 = x.lo / kStepTile;
-    x.n = x.kt + x.i1 / kStepTile - x.w0 + 1;
+    x.kt = (x.n_keep + TILE - 1) / TILE, x.w0 = x.lo / TILE;
+    x.n = x.kt + x.i1 / TILE - x.w0 + 1;
     return x;
+}
+
+// The tiles of a call lie in one row, head by head of every item, each with kBegin units of no work ahead of its tiles (what it costs to begin an item: queries, the warps'
+// sums).  CTA b of N has U / N of these units, and one more where b < U % N.
+constexpr int kBegin = 2;
+struct deal {
+    unsigned each, more;
+    __device__ __forceinline__ deal(unsigned U, unsigned N) : each(U / N), more(U - U / N * N) {}
+    __device__ __forceinline__ unsigned first(unsigned b) const { return b * each + min(b, more); }
+    __device__ __forceinline__ unsigned owner(unsigned u) const { return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each; }
+};
+// what a CTA works on at a time: tiles [tile, tile + n) of an item and head
+struct piece {
+    item it;
+    int entry, head, tile, n;
+    unsigned u; // the head's first unit
+};
+// the first piece from unit `at` on, which lies in the head that begins at x.u; n 0: none ahead of `end`
+template <int R, int TILE> __device__ __forceinline__ void piece_from(const attn_args &a, piece &x, unsigned at, unsigned end) {
+    for (;;) {
+        x.tile = max(0, (int)(at - x.u) - kBegin), x.n = (int)min((unsigned)(x.it.n + kBegin), end - x.u) - kBegin - x.tile;
+        if (x.n > 0) return;
+        x.n = 0, x.u += x.it.n + kBegin, at = x.u;
+        if (at >= end) return;
+        if (++x.head == a.G) {
+            x.head = 0;
+            do {
+                x.entry++;
+                x.it = item_of<R, TILE>(a, x.entry / a.groups, x.entry % a.groups);
+            } while (x.it.n == 0);
+        }
+    }
 }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -109,15 +140,19 @@ __device__ __forceinline__ uint32_t in_box(int byte) { return (uint32_t)(byte & 
 // P: numbers of a key and of a value, at most: 64, 128 or 256
 template <int CODE, int P, int NT, int PARTS> struct step_sizes {
     static constexpr int R = 8 * NT, KS = P / 16; // blocks of 16 value coordinates
-    static constexpr int min_ctas = (P <= 128 && NT == 1) || (P == 64 && NT == 2) ? 2 : 1;
+    // groups of 16 keys that a warp takes at once: two where the sums leave registers for them, which also gives the warp independent work.  Two CTAs of six warps an SM, or
+    // one of eight
+    static constexpr int min_ctas = P * NT <= 128 ? 2 : 1, W = min_ctas == 2 ? 6 : 8, U = P * NT <= 256 ? 2 : 1, threads = 32 * W, tile = 16 * W * U;
     // queries: int8 digits for steps of 32 numbers, or fp16 parts for steps of 16
     static constexpr bool digits = CODE == GGB_KV8_INT8;
     static constexpr int Q = digits ? PARTS + 2 : PARTS, QS = digits ? P / 32 : P / 16;
-    static constexpr int half = 16 * P, stage = 2 * half; // a warp's 16 keys, then their values; S of them on their way or in use
-    static constexpr int S = P == 256 ? 3 : P == 128 ? (NT == 1 ? 3 : 6) : min_ctas == 2 ? 6 : 8;
-    static constexpr size_t q_bytes = (size_t)Q * NT * QS * 256, ring_bytes = (size_t)kStepWarps * S * stage, red_bytes = (size_t)kStepWarps * R * P * 4;
-    static_assert(red_bytes <= ring_bytes && stage % 1024 == 0, "the warps' sums lie over the stages");
-    static constexpr size_t smem = 1024 + q_bytes + ring_bytes + (size_t)kStepWarps * (R * 8 + 768) + R * 8 + 64;
+    static constexpr int half = 16 * P, stage = 2 * half; // a group's keys, then their values; S of them on their way or in use
+    // the warps' sums of a piece meet beside the stages, on which the next piece's codes are arriving (16 rows of 256: no room, over them)
+    static constexpr bool beside = P == 64 || (P == 128 && NT > 1) || (P == 256 && NT == 1);
+    static constexpr int S = P == 256 ? (NT == 1 ? 2 : 3) : P == 128 ? (NT == 1 ? 4 : NT == 2 ? 4 : 2) : NT == 4 ? 7 : 4;
+    static constexpr size_t q_bytes = (size_t)Q * NT * QS * 256, ring_bytes = (size_t)W * S * stage, red_bytes = (size_t)W * R * P * 4;
+    static_assert((beside || red_bytes <= ring_bytes) && stage % 1024 == 0, "shared memory");
+    static constexpr size_t smem = 1024 + q_bytes + ring_bytes + (beside ? red_bytes : 0) + (size_t)W * (R * 8 + 768) + R * 8 + 64;
     static_assert((smem + 2048) * min_ctas <= 227 * 1024, "shared memory of an SM");
 };
 // where the pair of coordinates 2 i, 2 i + 1 of the 16 (P = 64: 8) numbers of lane group g lies in its row of the reduction, in pairs: rows of a warp's stores in different banks
@@ -186,136 +221,186 @@ template <int CODE, int P, int NT, int PARTS> __device__ __forceinline__ void st
 }
 
 template <int CODE, int P, int NT, int PARTS>
-__global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::min_ctas) kv8_step_kernel(const __grid_constant__ attn_args a, const __grid_constant__ line_maps maps) {
+__global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_sizes<CODE, P, NT, PARTS>::min_ctas) kv8_step_kernel(const __grid_constant__ attn_args a, const __grid_constant__ line_maps maps) {
     using Z = step_sizes<CODE, P, NT, PARTS>;
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
     constexpr int R = Z::R, KS = Z::KS, NB = P / 64, VW = P == 64 ? 2 : 4, VC = P == 256 ? 2 : 1; // words of a lane's piece of a value row, pieces
     extern __shared__ __align__(16) uint8_t ks_smem[];
-    __shared__ int64_t s_scan[kStepWarps], s_u, s_end, s_all;
-    __shared__ int s_dead, s_entry, s_head, s_tile;
-    __shared__ item s_it;
-    __shared__ __align__(8) uint64_t s_bars[kStepWarps * Z::S];
+    __shared__ unsigned s_scan[Z::W], s_end, s_all;
+    __shared__ int s_dead;
+    __shared__ piece s_piece[3]; // one whose sums are being taken, the next one (asked for meanwhile), the one behind that
+    __shared__ __align__(8) uint64_t s_bars[Z::W * Z::S];
     step_wait();
     volatile int *dead = &s_dead;
     const uint32_t raw = smem_u32(ks_smem), ring0 = (raw + 1023u) & ~1023u;
     uint8_t *base_at = ks_smem + (ring0 - raw);
-    float2 *red = reinterpret_cast<float2 *>(base_at); // over the stages
     uint2 *sq = reinterpret_cast<uint2 *>(base_at + Z::ring_bytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c4 = lane & 3;
     int2 *lines = reinterpret_cast<int2 *>(base_at + Z::ring_bytes + Z::q_bytes) + warp * 96; // [32]: lines of the tiles' keys and values
     float2 *scales = reinterpret_cast<float2 *>(lines + 32);                                  // [64]
-    float *sm = reinterpret_cast<float *>(base_at + Z::ring_bytes + Z::q_bytes + kStepWarps * 768), *sl = sm + kStepWarps * R, *srow = sl + kStepWarps * R;
+    float *sm = reinterpret_cast<float *>(base_at + Z::ring_bytes + Z::q_bytes + Z::W * 768), *sl = sm + Z::W * R, *srow = sl + Z::W * R;
     int *spos = reinterpret_cast<int *>(srow + R);
     float *svref = reinterpret_cast<float *>(spos + R);
+    float2 *red = reinterpret_cast<float2 *>(base_at + (Z::beside ? Z::ring_bytes + Z::q_bytes + Z::W * (768 + R * 8) + R * 8 + 64 : 0));
     const uint32_t ring = ring0 + warp * Z::S * Z::stage, bars = smem_u32(s_bars) + 8 * warp * Z::S;
     if (lane == 0)
         for (int k = 0; k < Z::S; k++) mbar_init(bars + 8 * k, 1);
     if (tid == 0) s_dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 
-    // ---- what this CTA has been dealt: units [u, end) of the tiles of all items, and where the first lies
+    // ---- what this CTA has been dealt
     if (a.part) {
-        const int entries = a.n_seq * a.groups, each = (entries + kStepThreads - 1) / kStepThreads, e0 = min(entries, tid * each), e1 = min(entries, e0 + each);
-        int64_t mine = 0, U = 0, base = 0;
-        for (int e = e0; e < e1; e++) mine += (int64_t)item_of<R>(a, e / a.groups, e % a.groups).n * a.G;
-        int64_t run = mine;
+        const int entries = a.n_seq * a.groups, each = (entries + Z::threads - 1) / Z::threads, e0 = min(entries, tid * each), e1 = min(entries, e0 + each);
+        unsigned mine = 0, U = 0, base = 0;
+        piece x;
+        for (x.entry = e0; x.entry < e1; x.entry++) {
+            x.it = item_of<R, Z::tile>(a, x.entry / a.groups, x.entry % a.groups);
+            if (x.it.n) mine += (x.it.n + kBegin) * a.G;
+        }
+        unsigned run = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int64_t x = __shfl_up_sync(0xffffffffu, run, off);
-            if (lane >= off) run += x;
+            const unsigned y = __shfl_up_sync(0xffffffffu, run, off);
+            if (lane >= off) run += y;
         }
         if (lane == 31) s_scan[warp] = run;
+        if (tid == 0) a.desc[2 * blockIdx.x] = make_int4(-1, 0, 0, 0), s_piece[0].n = 0;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kStepWarps; w++) {
+        for (int w = 0; w < Z::W; w++) {
             if (w < warp) base += s_scan[w];
             U += s_scan[w];
         }
-        const int64_t N = min((int64_t)gridDim.x, U), b = blockIdx.x;
-        if (tid == 0) a.desc[b] = make_int4(-1, 0, 0, 0);
-        if (b >= N) return;
-        const int64_t u = U * b / N;
+        const deal d(U, gridDim.x);
+        const unsigned u = d.first(blockIdx.x), end = d.first(blockIdx.x + 1);
         base += run - mine;
-        if (u >= base && u < base + mine) {
-            int e = e0;
-            item it;
-            for (;; e++) {
-                it = item_of<R>(a, e / a.groups, e % a.groups);
-                if (u < base + (int64_t)it.n * a.G) break;
-                base += (int64_t)it.n * a.G;
-            }
-            s_it = it, s_entry = e, s_head = (int)((u - base) / it.n), s_tile = (int)((u - base) % it.n);
-            s_u = u, s_end = U * (b + 1) / N, s_all = U;
+        if (u < end && u >= base && u < base + mine) {
+            if (each > 1)
+                for (x.entry = e0;; x.entry++) {
+                    x.it = item_of<R, Z::tile>(a, x.entry / a.groups, x.entry % a.groups);
+                    const unsigned n = x.it.n ? (x.it.n + kBegin) * a.G : 0;
+                    if (u < base + n) break;
+                    base += n;
+                }
+            else x.entry = e0;
+            x.head = (int)((u - base) / (unsigned)(x.it.n + kBegin)), x.u = base + x.head * (x.it.n + kBegin);
+            piece_from<R, Z::tile>(a, x, u, end);
+            s_piece[0] = x, s_end = end, s_all = U;
         }
     } else if (tid == 0) {
-        s_entry = blockIdx.x / a.G, s_head = blockIdx.x - s_entry * a.G, s_tile = 0;
-        s_it = item_of<R>(a, s_entry / a.groups, s_entry % a.groups);
-        s_u = 0, s_end = s_it.n, s_all = 0;
+        piece x;
+        x.entry = blockIdx.x / a.G, x.head = blockIdx.x - x.entry * a.G, x.tile = 0, x.u = 0;
+        x.it = item_of<R, Z::tile>(a, x.entry / a.groups, x.entry % a.groups);
+        x.n = x.it.n;
+        s_piece[0] = x, s_end = 0, s_all = 0;
     }
     __syncthreads();
-
-    int stage = 0; // stages are asked for and used in turn
+    const int hpg = a.H / a.G;
+    auto write_following = [&](int from, int to) { // one thread
+        piece x = s_piece[from];
+        const unsigned at = x.u + kBegin + x.tile + x.n;
+        const bool more = x.n > 0 && at < s_end;
+        x.n = 0;
+        if (more) piece_from<R, Z::tile>(a, x, at, s_end);
+        s_piece[to] = x;
+    };
+    auto stage_queries = [&](const piece &x) {
+        for (int r = warp; r < R; r += Z::W) {
+            const int row = x.it.row0 + r, tq = row / hpg, h = x.head * hpg + (row - tq * hpg);
+            stage_row<CODE, P, NT, PARTS>(a, a.q + ((x.it.t0 + tq) * a.H + h) * a.D, r < x.it.rows, r, sq, srow);
+            if (lane == 0) spos[r] = r < x.it.rows ? x.it.p0 + tq : -1; // sees nothing
+        }
+    };
+    auto fetch_queries = [&](const piece &x) { // to the cache, ahead of that
+        for (int r = warp; r < x.it.rows; r += Z::W) {
+            const int row = x.it.row0 + r, tq = row / hpg, h = x.head * hpg + (row - tq * hpg);
+            if (4 * lane < a.D) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.q + ((x.it.t0 + tq) * a.H + h) * a.D + 4 * lane));
+        }
+    };
+    // where a lane's pieces lie in a stage (behind the end of a row: the row's first piece, which meets zeros of the queries or leaves by no coordinate)
+    uint32_t k_at[2][NB], v_at[4][VC];
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            k_at[e][b] = in_box((g8 + 8 * e) * a.D + (64 * b + 16 * c4 < a.D ? 64 * b + 16 * c4 : 0));
+            asm volatile("" : "+r"(k_at[e][b])); // computed once
+        }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int c = 0; c < VC; c++) {
+            v_at[e][c] = Z::half + in_box((2 * c4 + (e & 1) + 8 * (e >> 1)) * a.Dv + (128 * c + 4 * VW * g8 < a.Dv ? 128 * c + 4 * VW * g8 : 0));
+            asm volatile("" : "+r"(v_at[e][c]));
+        }
+    // stages are asked for and used in turn: `asked` and `used` groups so far; of the piece that is asked for, groups [ask_k, ask_n) are left
+    int asked = 0, used = 0, ask_stage = 0, stage = 0, ask_slot = 0, ask_k = 0, ask_n = Z::U * s_piece[0].n;
     uint32_t parity = 0;
-    while (s_u < s_end) {
-        // ---- a piece of an item: its tiles [tile, tile + n)
-        const int hpg = a.H / a.G, head = s_head, tile = s_tile, n = (int)min((int64_t)(s_it.n - tile), s_end - s_u);
-        // the 16 positions of this warp in a tile.  32 tiles at a time, a lane each, are looked up: the lines of a group's keys (-1: no row sees any of it) and
-        // values, the scales of both (-1, too)
-        auto first_of = [&](int t) { return (t < s_it.kt ? t : s_it.w0 + t - s_it.kt) * kStepTile + 16 * warp; };
-        auto ask = [&](int k, int at_stage) {
-            if ((k & 31) == 0) {
-                const int t = tile + k + lane, first = first_of(t);
+    // the first of this warp's positions in a tile
+    auto first_of = [&](const item &it, int t) { return (t < it.kt ? t : it.w0 + t - it.kt) * Z::tile + 16 * Z::U * warp; };
+    // Asks for whatever stages are free, for the piece in `slot` and the next one.  32 groups at a time, a lane each, are looked up: the lines of a group's keys (-1: no row
+    // sees any of it) and values; the scales of both (-1, too) are on their way to registers until keep_scale()
+    float2 scale = make_float2(0.f, 0.f);
+    int scale_at = -1;
+    auto keep_scale = [&] {
+        if (scale_at >= 0) scales[scale_at] = scale;
+        scale_at = -1;
+        __syncwarp();
+    };
+    auto ask = [&](int slot, bool next) {
+        while (asked - used < Z::S) {
+            if (ask_k == ask_n) {
+                const int then = slot == 2 ? 0 : slot + 1;
+                if (!next || ask_slot != slot || s_piece[then].n == 0) break;
+                ask_slot = then, ask_k = 0, ask_n = Z::U * s_piece[then].n;
+            }
+            if (*dead) break; // a wait has run out: no more requests
+            if ((ask_k & 31) == 0) {
+                keep_scale();
+                scale = make_float2(-1.f, 0.f), scale_at = (asked + lane) & 63;
+                const piece &x = s_piece[ask_slot];
+                const int t = x.tile + (ask_k + lane) / Z::U, first = first_of(x.it, t) + 16 * ((ask_k + lane) % Z::U);
                 int2 line = make_int2(-1, 0);
-                float2 scale = make_float2(-1.f, 0.f);
-                if (k + lane < n && (t < s_it.kt ? first < s_it.n_keep : first + 15 >= s_it.lo && first <= s_it.i1)) {
+                if (ask_k + lane < ask_n && (t < x.it.kt ? first < x.it.n_keep : first + 15 >= x.it.lo && first <= x.it.i1)) {
                     const int pg = first / a.B, grp = (first - pg * a.B) / kKv8Group;
-                    const int64_t rec = (int64_t)a.tables[s_it.s * a.table_ld + pg] * a.G + head;
+                    const int64_t rec = (int64_t)a.tables[x.it.s * a.table_ld + pg] * a.G + x.head;
                     const float *sc = reinterpret_cast<const float *>(a.cache + rec * a.record + a.B * (a.D + a.Dv)) + grp;
                     line.x = (int)(rec * (a.record / 128)) + grp * (a.D / 8);
                     line.y = (int)(rec * (a.record / 128)) + a.B / kKv8Group * (a.D / 8) + grp * (a.Dv / 8);
                     scale = make_float2(sc[0], sc[a.B / kKv8Group]);
                 }
-                scales[(k + lane) & 63] = scale, lines[lane] = line;
+                lines[lane] = line;
                 __syncwarp();
             }
-            if (lane == 0) {
-                const int2 line = lines[k & 31];
-                const uint32_t to = ring + at_stage * Z::stage, bar = bars + 8 * at_stage;
-                if (line.x >= 0) request(maps, to, to + Z::half, line.x, line.y, 16 * (a.D + a.Dv), bar);
-                else mbar_arrive(bar);
-            }
-        };
-        // tiles [whole0, whole0 + wholes) of the window: every row sees all 16 positions
-        const int up = s_it.i0 - 15 - 16 * warp, down = max(s_it.lo, a.window > 0 ? (int)max((int64_t)0, s_it.i1 - a.window + 1) : 0) - 16 * warp;
-        const int whole0 = s_it.kt + max(0, (down + kStepTile - 1) / kStepTile - s_it.w0), wholes = up < 0 ? 0 : max(0, s_it.kt + up / kStepTile - s_it.w0 - whole0 + 1);
+            do {
+                if (lane == 0) {
+                    const int2 line = lines[ask_k & 31];
+                    const uint32_t to = ring + ask_stage * Z::stage, bar = bars + 8 * ask_stage;
+                    if (line.x >= 0) request(maps, to, to + Z::half, line.x, line.y, 16 * (a.D + a.Dv), bar);
+                    else mbar_arrive(bar);
+                }
+                asked++, ask_k++;
+                if (++ask_stage == Z::S) ask_stage = 0;
+            } while (asked - used < Z::S && ask_k < ask_n && (ask_k & 31) != 0);
+        }
+    };
+    if (s_piece[0].n > 0) {
+        fetch_queries(s_piece[0]);
+        ask(0, false); // (the piece behind it is not known yet)
+        stage_queries(s_piece[0]);
+    }
+    if (tid == Z::threads - 1) write_following(0, 1);
+    __syncthreads();
+    for (int slot = 0; s_piece[slot].n > 0; slot = slot == 2 ? 0 : slot + 1) {
+        // ---- a piece of an item: its tiles [tile, tile + n)
+        const item &s_it = s_piece[slot].it;
+        const int tile = s_piece[slot].tile, n = s_piece[slot].n;
+        if (ask_slot != slot) ask_slot = slot, ask_k = 0, ask_n = Z::U * n; // (nothing of it has been asked for)
+        // tiles [whole0, whole0 + wholes) of the window: every row sees all of this warp's positions
+        constexpr int last_of = 16 * Z::U - 1;
+        const int up = s_it.i0 - last_of - 16 * Z::U * warp, down = max(s_it.lo, a.window > 0 ? (int)max((int64_t)0, s_it.i1 - a.window + 1) : 0) - 16 * Z::U * warp;
+        const int whole0 = s_it.kt + max(0, (down + Z::tile - 1) / Z::tile - s_it.w0), wholes = up < 0 ? 0 : max(0, s_it.kt + up / Z::tile - s_it.w0 - whole0 + 1);
 
-        // where a lane's pieces lie in a stage (behind the end of a row: the row's first piece, which meets zeros of the queries or leaves by no coordinate)
-        uint32_t k_at[2][NB], v_at[4][VC];
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                k_at[e][b] = in_box((g8 + 8 * e) * a.D + (64 * b + 16 * c4 < a.D ? 64 * b + 16 * c4 : 0));
-                asm volatile("" : "+r"(k_at[e][b])); // computed once
-            }
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int c = 0; c < VC; c++) {
-                v_at[e][c] = Z::half + in_box((2 * c4 + (e & 1) + 8 * (e >> 1)) * a.Dv + (128 * c + 4 * VW * g8 < a.Dv ? 128 * c + 4 * VW * g8 : 0));
-                asm volatile("" : "+r"(v_at[e][c]));
-            }
-        bool lost = *dead != 0; // a wait has run out: no more requests
-        for (int k = 0, s = stage; k < Z::S && k < n && !lost; k++) {
-            ask(k, s);
-            if (++s == Z::S) s = 0;
-        }
-        for (int r = warp; r < R; r += kStepWarps) {
-            const int row = s_it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
-            stage_row<CODE, P, NT, PARTS>(a, a.q + ((s_it.t0 + tq) * a.H + h) * a.D, r < s_it.rows, r, sq, srow);
-            if (lane == 0) spos[r] = r < s_it.rows ? s_it.p0 + tq : -1; // sees nothing
-        }
-        __syncthreads();
         float rowf[NT][2], m[NT][2], l[NT][2], o[KS][NT][4], vref = 0.f, vinv = 0.f;
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -328,15 +413,27 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[i][t][e] = 0.f;
 
-        for (int k = 0; k < n && !lost; k++) {
-            if (!mbar_wait_warp(bars + 8 * stage, parity, dead)) break;
-            const float2 sc = scales[k & 63];
-            if (sc.x >= 0.f) {
-                const uint32_t from = ring + stage * Z::stage;
-                float z[NT][4];
+        for (int k = 0;; k++) {
+            ask(slot, Z::beside);
+            if (k == n) break;
+            if (scale_at >= 0) keep_scale();
+            bool here = true;
+            uint32_t from[Z::U];
+            float2 sc[Z::U];
+#pragma unroll
+            for (int u = 0; u < Z::U; u++) {
+                here = here && mbar_wait_warp(bars + 8 * stage, parity, dead);
+                from[u] = ring + stage * Z::stage, sc[u] = scales[(used + u) & 63];
+                if (++stage == Z::S) stage = 0, parity ^= 1;
+            }
+            if (!here) break;
+            // ---- scores
+            float z[Z::U][NT][4];
+#pragma unroll
+            for (int u = 0; u < Z::U; u++) {
                 uint4 kw[2][NB];
 #pragma unroll
-                for (int b = 0; b < NB; b++) kw[0][b] = lds_u4(from + k_at[0][b]), kw[1][b] = lds_u4(from + k_at[1][b]);
+                for (int b = 0; b < NB; b++) kw[0][b] = lds_u4(from[u] + k_at[0][b]), kw[1][b] = lds_u4(from[u] + k_at[1][b]);
                 if (Z::digits) {
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
@@ -352,8 +449,8 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
                             }
 #pragma unroll
                         for (int e = 0; e < 4; e++) // whole numbers below 2^29 each
-                            z[t][e] = Z::Q == 3 ? fmaf((float)(zi[2][e] * 128 + zi[1][e]), 128.f, (float)zi[0][e])
-                                                : fmaf((float)(zi[Z::Q - 1][e] * 128 + zi[Z::Q - 2][e]), 16384.f, (float)(zi[1][e] * 128 + zi[0][e]));
+                            z[u][t][e] = Z::Q == 3 ? fmaf((float)(zi[2][e] * 128 + zi[1][e]), 128.f, (float)zi[0][e])
+                                                   : fmaf((float)(zi[Z::Q - 1][e] * 128 + zi[Z::Q - 2][e]), 16384.f, (float)(zi[1][e] * 128 + zi[0][e]));
                     }
                 } else {
 #pragma unroll
@@ -369,102 +466,118 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
 #pragma unroll
                                 for (int t = 0; t < NT; t++) {
                                     const uint2 y = sq[((part * NT + t) * Z::QS + 4 * b + w) * 32 + lane];
-                                    if (b + w == 0 && part == PARTS - 1) mma16816_first(z[t], a0, a1, a2, a3, y.x, y.y);
-                                    else mma16816(z[t], a0, a1, a2, a3, y.x, y.y);
+                                    if (b + w == 0 && part == PARTS - 1) mma16816_first(z[u][t], a0, a1, a2, a3, y.x, y.y);
+                                    else mma16816(z[u][t], a0, a1, a2, a3, y.x, y.y);
                                 }
                         }
                     }
                 }
-                // ---- weights
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) z[t][e] *= rowf[t][e & 1] * sc.x;
-                if (a.cap > 0.f) {
+                    for (int e = 0; e < 4; e++) z[u][t][e] *= rowf[t][e & 1] * sc[u].x;
+            }
+            if (a.cap > 0.f) {
+#pragma unroll
+                for (int u = 0; u < Z::U; u++)
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) z[t][e] = a.cap * kLog2e * tanhf(z[t][e] / a.cap);
-                }
-                if ((unsigned)(tile + k - whole0) >= (unsigned)wholes) {
-                    const int now = tile + k, first = first_of(now), i1 = s_it.i1;
-                    const int lo = now < s_it.kt ? 0 : s_it.lo, hi = now < s_it.kt ? s_it.n_keep - 1 : i1;
+                        for (int e = 0; e < 4; e++) z[u][t][e] = a.cap * kLog2e * tanhf(z[u][t][e] / a.cap);
+            }
+            if ((unsigned)(tile + k - whole0) >= (unsigned)wholes) {
+                const int now = tile + k, i1 = s_it.i1, lo = now < s_it.kt ? 0 : s_it.lo, hi = now < s_it.kt ? s_it.n_keep - 1 : i1;
+#pragma unroll
+                for (int u = 0; u < Z::U; u++) {
+                    const int first = first_of(s_it, now) + 16 * u;
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int j = first + g8 + 8 * (e >> 1), i = spos[8 * t + 2 * c4 + (e & 1)];
-                            if (!(j >= lo && j <= hi && j <= i && (a.window <= 0 || i - j < a.window || j < a.keep))) z[t][e] = -INFINITY;
+                            if (!(j >= lo && j <= hi && j <= i && (a.window <= 0 || i - j < a.window || j < a.keep))) z[u][t][e] = -INFINITY;
                         }
-                    // behind the last position there may be e4m3 codes that are no numbers, whose weight of zero would spoil a sum
-                    if (CODE == GGB_KV8_E4M3 && first + 15 > i1) {
+                    // behind the last position, and where nothing was asked for, there may be e4m3 codes that are no numbers, whose weight of zero would spoil a sum
+                    if (CODE == GGB_KV8_E4M3 && (first + 15 > i1 || sc[u].x < 0.f)) {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (first + 2 * c4 + (e & 1) + 8 * (e >> 1) > i1)
+                            if (first + 2 * c4 + (e & 1) + 8 * (e >> 1) > i1 || sc[u].x < 0.f)
 #pragma unroll
                                 for (int c = 0; c < VC; c++) {
-                                    asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c]), "r"(0u) : "memory");
-                                    if (VW == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from + v_at[e][c] + 8), "r"(0u) : "memory");
+                                    asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from[u] + v_at[e][c]), "r"(0u) : "memory");
+                                    if (VW == 4) asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(from[u] + v_at[e][c] + 8), "r"(0u) : "memory");
                                 }
                         fence_async_smem();
                         __syncwarp();
                     }
                 }
-                bool grow = sc.y > 64.f * vref;
+            }
+            // ---- weights
+            float vmost = sc[0].y;
+            bool grow = false;
+#pragma unroll
+            for (int u = 0; u < Z::U; u++) {
+                vmost = fmaxf(vmost, sc[u].y);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) grow |= z[t][e] > m[t][e & 1] + 8.f;
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float vnew = sc.y > 64.f * vref ? sc.y : vref, vf = vnew > 0.f ? vref / vnew : 0.f;
-                    vref = vnew, vinv = vnew > 0.f ? 1.f / vnew : 0.f;
+                    for (int e = 0; e < 4; e++) grow |= z[u][t][e] > m[t][e & 1] + 8.f;
+            }
+            if (__any_sync(0xffffffffu, grow || vmost > 64.f * vref)) {
+                const float vnew = vmost > 64.f * vref ? vmost : vref, vf = vnew > 0.f ? vref / vnew : 0.f;
+                vref = vnew, vinv = vnew > 0.f ? 1.f / vnew : 0.f;
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float x = fmaxf(z[t][e], z[t][e + 2]);
+                    for (int e = 0; e < 2; e++) {
+                        float x = fmaxf(fmaxf(z[0][t][e], z[0][t][e + 2]), fmaxf(z[Z::U - 1][t][e], z[Z::U - 1][t][e + 2]));
 #pragma unroll
-                            for (int off = 4; off <= 16; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                            x = fmaxf(x, m[t][e]);
-                            const float f = exp2f(m[t][e] - x);
-                            m[t][e] = x;
-                            l[t][e] *= f;
+                        for (int off = 4; off <= 16; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+                        x = fmaxf(x, m[t][e]);
+                        const float f = exp2f(m[t][e] - x);
+                        m[t][e] = x;
+                        l[t][e] *= f;
 #pragma unroll
-                            for (int i = 0; i < KS; i++) o[i][t][e] *= f * vf, o[i][t][e + 2] *= f * vf;
-                        }
-                }
-                const float vrel = sc.y * vinv;
-                uint32_t pb[PARTS][NT][2];
+                        for (int i = 0; i < KS; i++) o[i][t][e] *= f * vf, o[i][t][e + 2] *= f * vf;
+                    }
+            }
+            uint32_t pb[Z::U][PARTS][NT][2];
+#pragma unroll
+            for (int u = 0; u < Z::U; u++) {
+                const float vrel = sc[u].y * vinv;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        w[e] = ex2_approx(z[t][e] - m[t][e & 1]);
+                        w[e] = ex2_approx(z[u][t][e] - m[t][e & 1]);
                         l[t][e & 1] += w[e];
                         w[e] *= vrel;
                     }
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
                         const uint32_t hi = half2_bits(w[2 * y], w[2 * y + 1]);
-                        pb[0][t][y] = turn8x8(hi);
+                        pb[u][0][t][y] = turn8x8(hi);
                         if (PARTS == 2) {
                             const float2 back = half2_floats(hi);
-                            pb[PARTS - 1][t][y] = turn8x8(half2_bits(w[2 * y] - back.x, w[2 * y + 1] - back.y));
+                            pb[u][PARTS - 1][t][y] = turn8x8(half2_bits(w[2 * y] - back.x, w[2 * y + 1] - back.y));
                         }
                     }
                 }
-                // ---- output: coordinates 2 i, 2 i + 1 of a lane's piece are rows g8 and g8 + 8 of block i
+            }
+            // ---- output: coordinates 2 i, 2 i + 1 of a lane's piece are rows g8 and g8 + 8 of block i
+#pragma unroll
+            for (int u = 0; u < Z::U; u++)
 #pragma unroll
                 for (int c = 0; c < VC; c++) {
                     uint32_t vx[4][VW];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         if (VW == 4) {
-                            const uint4 x = lds_u4(from + v_at[e][c]);
+                            const uint4 x = lds_u4(from[u] + v_at[e][c]);
                             vx[e][0] = x.x, vx[e][1] = x.y, vx[e][VW - 2] = x.z, vx[e][VW - 1] = x.w;
                         } else {
-                            const uint2 x = lds_u2(from + v_at[e][c]);
+                            const uint2 x = lds_u2(from[u] + v_at[e][c]);
                             vx[e][0] = x.x, vx[e][1] = x.y;
                         }
                     }
@@ -479,17 +592,15 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
 #pragma unroll
                             for (int part = PARTS - 1; part >= 0; part--)
 #pragma unroll
-                                for (int t = 0; t < NT; t++) mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[part][t][0], pb[part][t][1]);
+                                for (int t = 0; t < NT; t++) mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[u][part][t][0], pb[u][part][t][1]);
                         }
                 }
-            }
+            used += Z::U;
             __syncwarp();
-            if (k + Z::S < n) ask(k + Z::S, stage); // what has been used
-            if (++stage == Z::S) stage = 0, parity ^= 1;
         }
 
         // ---- the warps' sums meet
-        __syncthreads(); // (every group that was asked for has been used)
+        if (!Z::beside) __syncthreads(); // (every group that was asked for has been used)
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -506,19 +617,19 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
         __syncthreads();
         const bool whole_item = n == s_it.n;
         float *part = a.part ? a.part + ((int64_t)blockIdx.x * 2 + (tile == 0)) * R * (a.Dv + 2) : nullptr;
-        constexpr int TPR = kStepThreads / R; // threads a row
+        constexpr int TPR = Z::threads / R; // threads a row
         const int r = tid / TPR;
         if (r < s_it.rows) {
-            float M = -INFINITY, L = 0.f, f[kStepWarps];
+            float M = -INFINITY, L = 0.f, f[Z::W];
 #pragma unroll
-            for (int w = 0; w < kStepWarps; w++) M = fmaxf(M, sm[w * R + r]);
+            for (int w = 0; w < Z::W; w++) M = fmaxf(M, sm[w * R + r]);
 #pragma unroll
-            for (int w = 0; w < kStepWarps; w++) {
+            for (int w = 0; w < Z::W; w++) {
                 f[w] = exp2f(sm[w * R + r] - M);
                 L = fmaf(sl[w * R + r], f[w], L);
                 f[w] *= svref[w];
             }
-            const int row = s_it.row0 + r, tq = row / hpg, h = head * hpg + (row - tq * hpg);
+            const int row = s_it.row0 + r, tq = row / hpg, h = s_piece[slot].head * hpg + (row - tq * hpg);
             const int64_t t = s_it.t0 + tq;
             const row_end end(a, h, M, L);
             for (int pr = tid - r * TPR; pr < a.Dv / 2; pr += TPR) {
@@ -526,7 +637,7 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
                 const int at = 64 * (pr / 64) + red_at<P>((pr % 64) / W, pr % W, (r % 8) / 2);
                 float2 y = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kStepWarps; w++) {
+                for (int w = 0; w < Z::W; w++) {
                     const float2 x = red[(w * R + r) * (P / 2) + at];
                     y.x = fmaf(x.x, f[w], y.x), y.y = fmaf(x.y, f[w], y.y);
                 }
@@ -540,23 +651,17 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
             }
             if (!whole_item && tid == r * TPR) part[(int64_t)r * (a.Dv + 2) + a.Dv] = M, part[(int64_t)r * (a.Dv + 2) + a.Dv + 1] = L;
         }
-        if (!whole_item && tile == 0 && tid == 0) { // it ends with the CTA that has its last tile
-            const int64_t N = min((int64_t)gridDim.x, s_all), last = s_u - tile + s_it.n - 1;
-            a.desc[blockIdx.x] = make_int4(s_it.s, s_it.rg, head, (int)(((last + 1) * N - 1) / s_all));
+        if (!whole_item && tile + n < s_it.n && tid == 0) { // joined by the CTAs that have it but for the last, whose own last piece may be another one's
+            const piece &x = s_piece[slot];
+            const deal d(s_all, gridDim.x);
+            a.desc[2 * blockIdx.x] = make_int4(x.it.s, x.it.rows, x.head, x.it.row0);
+            a.desc[2 * blockIdx.x + 1] = make_int4((int)d.owner(x.u + kBegin), (int)d.owner(x.u + kBegin + x.it.n - 1), (int)x.it.t0, 0);
         }
-        fence_async_smem();
-        __syncthreads(); // what is read above is written by the next piece, sums by its copies
-        if (tid == 0) {
-            s_u += n, s_tile = 0;
-            if (s_u < s_end && ++s_head == a.G) {
-                s_head = 0;
-                do {
-                    s_entry++;
-                    s_it = item_of<R>(a, s_entry / a.groups, s_entry % a.groups);
-                } while (s_it.n == 0);
-            }
-        }
-        __syncthreads();
+        const int then = slot == 2 ? 0 : slot + 1, last = then == 2 ? 0 : then + 1;
+        if (s_piece[then].n > 0) stage_queries(s_piece[then]);
+        if (tid == Z::threads - 1) write_following(then, last);
+        if (!Z::beside) fence_async_smem(); // sums are written over by copies
+        __syncthreads();                    // and by sums
     }
     if (warp == 0) {
         settle(dead);
@@ -564,60 +669,81 @@ __global__ void __launch_bounds__(kStepThreads, step_sizes<CODE, P, NT, PARTS>::
     }
 }
 
-// an item's pieces: a row a CTA.  Threads of a column (four numbers) have the pieces in turn and are added up in order
+// an item's pieces, by the CTAs of the same numbers as those that hold them, all but the last: a share of the item's numbers each.  Threads of a column of four numbers have
+// the pieces in turn, four of them asked for ahead of the rows' maxima and sums, and are added up in order
 template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ attn_args a) {
     __shared__ float4 s_y[256];
-    __shared__ float s_f[kMaxCtas], s_red[8], s_l[8];
+    __shared__ float s_f[3 * kMaxCtas], s_g[3 * kMaxCtas], s_m[R], s_l[R];
     step_wait();
-    const int b0 = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int4 d = a.desc[b0];
+    const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
     if (d.x < 0) return;
-    const int hpg = a.H / a.G, row = d.y * R + r, tq = row / hpg, h = d.z * hpg + (row - tq * hpg), pieces = d.w - b0 + 1;
-    const int64_t t = a.starts[d.x] + tq;
-    if (t >= a.starts[d.x + 1]) return;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hpg = a.H / a.G, b0 = e.x, pieces = e.y - b0 + 1, share = blockIdx.x - b0, shares = pieces - 1;
     const int64_t pitch = a.Dv + 2;
-    auto piece = [&](int k) { return a.part + (((int64_t)(b0 + k) * 2 + (k == 0)) * R + r) * pitch; };
-    float M = -INFINITY;
-    for (int k = tid; k < pieces; k += 256) M = fmaxf(M, s_f[k] = piece(k)[a.Dv]);
-    M = warp_max_f32(M);
-    if (lane == 0) s_red[warp] = M;
-    __syncthreads();
+    const int quads = a.Dv / 4, rows = d.y, q0 = rows * quads * share / shares, q1 = rows * quads * (share + 1) / shares, r0 = q0 / quads;
+    if (q0 == q1) return;
+    const int nq = min(256, q1 - q0), ways = 256 / nq, way = tid / nq;
+    auto piece = [&](int k, int r) { return a.part + (((int64_t)(b0 + k) * 2 + (k == 0)) * R + r) * pitch; };
+    float4 ahead[4];
+    auto load = [&](int k, int r, int c) {
+        const float2 *x = reinterpret_cast<const float2 *>(piece(k, r) + c);
+        const float2 p = x[0], s = x[1];
+        return make_float4(p.x, p.y, s.x, s.y);
+    };
+    int q = q0 + tid - way * nq;
 #pragma unroll
-    for (int w = 0; w < 8; w++) M = fmaxf(M, s_red[w]);
-    float L = 0.f;
-    for (int k = tid; k < pieces; k += 256) {
-        const float f = exp2f(s_f[k] - M);
-        L = fmaf(piece(k)[a.Dv + 1], f, L);
-        s_f[k] = f;
-    }
-    L = warp_sum_f32(L);
-    if (lane == 0) s_l[warp] = L;
-    __syncthreads();
-    L = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; w++) L += s_l[w];
-    const int quads = a.Dv / 4, ways = 256 / quads, way = tid / quads, c = 4 * (tid - way * quads);
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (way < ways)
-#pragma unroll 4
-        for (int k = way; k < pieces; k += ways) {
-            const float2 *x = reinterpret_cast<const float2 *>(piece(k) + c);
-            const float2 p = x[0], q = x[1];
-            const float f = s_f[k];
-            y.x = fmaf(p.x, f, y.x), y.y = fmaf(p.y, f, y.y), y.z = fmaf(q.x, f, y.z), y.w = fmaf(q.y, f, y.w);
+    for (int u = 0; u < 4; u++)
+        if (way < ways && way + u * ways < pieces) ahead[u] = load(way + u * ways, q / quads, 4 * (q % quads));
+    for (int r = r0 + warp; r <= (q1 - 1) / quads; r += 8) {
+        float *f = s_f + (r - r0) * pieces, *g = s_g + (r - r0) * pieces, M = kNone, L = 0.f;
+#pragma unroll 8
+        for (int k = lane; k < pieces; k += 32) {
+            const float2 ml = *reinterpret_cast<const float2 *>(piece(k, r) + a.Dv);
+            M = fmaxf(M, f[k] = ml.x);
+            g[k] = ml.y;
         }
-    s_y[tid] = y;
-    __syncthreads();
-    if (way != 0) return;
-    for (int w = 1; w < ways; w++) {
-        const float4 x = s_y[w * quads + tid];
-        y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+        M = warp_max_f32(M);
+        for (int k = lane; k < pieces; k += 32) L = fmaf(g[k], f[k] = exp2f(f[k] - M), L);
+        L = warp_sum_f32(L);
+        if (lane == 0) s_m[r - r0] = M, s_l[r - r0] = L;
     }
-    const row_end end(a, h, M, L);
-    const int64_t to = (int64_t)h * a.Dv + c;
-    E *out = reinterpret_cast<E *>(a.out) + t * a.H * a.Dv + to;
-    out[0] = from_f32<E>(gated(a, y.x * end.f, t, to)), out[1] = from_f32<E>(gated(a, y.y * end.f, t, to + 1));
-    out[2] = from_f32<E>(gated(a, y.z * end.f, t, to + 2)), out[3] = from_f32<E>(gated(a, y.w * end.f, t, to + 3));
+    __syncthreads();
+    for (; q < q1 && (way == 0 || ways > 1); q += nq) {
+        const int r = q / quads, c = 4 * (q - r * quads);
+        const float *f = s_f + (r - r0) * pieces;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (way < ways) {
+            auto add = [&](const float4 &x, float g) { y.x = fmaf(x.x, g, y.x), y.y = fmaf(x.y, g, y.y), y.z = fmaf(x.z, g, y.z), y.w = fmaf(x.w, g, y.w); };
+            int k = way;
+            if (q < q0 + nq) {
+#pragma unroll
+                for (int u = 0; u < 4; u++, k += ways)
+                    if (k < pieces) add(ahead[u], f[k]);
+            }
+#pragma unroll 4
+            for (; k < pieces; k += ways) add(load(k, r, c), f[k]);
+        }
+        if (ways > 1) { // (then there is one q a thread)
+            auto add_way = [&](int w) {
+                const float4 x = s_y[w * nq + (q - q0)];
+                y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+            };
+            s_y[tid] = y;
+            __syncthreads();
+            if (way < 8)
+                for (int w = way + 8; w < ways; w += 8) add_way(w);
+            __syncthreads();
+            s_y[tid] = y;
+            __syncthreads();
+            if (way != 0) return;
+            for (int w = 1; w < min(8, ways); w++) add_way(w);
+        }
+        const int row = d.w + r, tq = row / hpg, h = d.z * hpg + (row - tq * hpg);
+        const int64_t t = e.z + tq, to = (int64_t)h * a.Dv + c;
+        const row_end end(a, h, s_m[r - r0], s_l[r - r0]);
+        E *out = reinterpret_cast<E *>(a.out) + t * a.H * a.Dv + to;
+        out[0] = from_f32<E>(gated(a, y.x * end.f, t, to)), out[1] = from_f32<E>(gated(a, y.y * end.f, t, to + 1));
+        out[2] = from_f32<E>(gated(a, y.z * end.f, t, to + 2)), out[3] = from_f32<E>(gated(a, y.w * end.f, t, to + 3));
+    }
 }
 
 template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64_t max_new) {
@@ -625,6 +751,7 @@ template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
     const int64_t groups = (max_new * (a.H / a.G) + Z::R - 1) / Z::R;
     GGB_CHECK_ARG(max_new * (a.H / a.G) < (1ll << 30) && a.n_seq * groups * a.G < (1ll << 31), "kv8_attn: too many sequences, tokens and heads for a launch");
+    GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.table_ld * a.B + a.keep) / Z::tile + 4) < (1ll << 31), "kv8_attn: too many positions for a launch"); // the units of a deal, at most
     a.groups = (int)groups;
     auto k = kv8_step_kernel<CODE, P, NT, PARTS>;
     int rc = ggb_allow_smem(k, Z::smem);
@@ -634,10 +761,10 @@ template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64
     rc = ggb_tensor_map_bf16(&maps.k, a.cache, (1ll << 31) - 1, 64, 64, a.D / 8);
     if (!rc) rc = ggb_tensor_map_bf16(&maps.v, a.cache, (1ll << 31) - 1, 64, 64, a.Dv / 8);
     if (rc) return rc;
-    GGB_CUDA(ggb_launch_step(k, dim3(ctas), dim3(kStepThreads), Z::smem, a, maps));
+    GGB_CUDA(ggb_launch_step(k, dim3(ctas), dim3(Z::threads), Z::smem, a, maps));
     GGB_LAUNCH_CHECK();
     if (a.part) {
-        GGB_CUDA(ggb_launch_step(kv8_join_kernel<Z::R, E>, dim3(ctas, Z::R), dim3(256), 0, a));
+        GGB_CUDA(ggb_launch_step(kv8_join_kernel<Z::R, E>, dim3(ctas), dim3(256), 0, a));
         GGB_LAUNCH_CHECK();
     }
     return GGB_OK;
