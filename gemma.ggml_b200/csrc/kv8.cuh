@@ -66,9 +66,10 @@ struct attn_args {
     int64_t ldg, record;
     void *out;
     int groups;     // items of a sequence and key head, at most
+    int64_t rows_above, rows_up_to; // sequences of more rows (tokens x query heads of a key head) than the one, up to the other, are this kernel's
     float *part;    // [CTA][2][rows][Dv + 2], or null: an item a CTA
     int4 *desc;     // [CTA][2], of an item that begins or goes on here and ends elsewhere: sequence (or -1), rows, key head, first row; first and last CTA that have it, first token
-    int vec_q;      // queries begin on a 16-byte boundary
+    int vec_q, vec_out; // queries, results begin on a 16-byte boundary
     int *wait_error;
 };
 // four codes as two pairs of fp16 numbers.  int8: code + 128 behind the bits of 1024, less 1152
@@ -107,6 +108,61 @@ struct row_end {
     }
 };
 __device__ __forceinline__ float gated(const attn_args &a, float y, int64_t t, int64_t at) { return a.gate ? y / (1.f + expf(-a.gate[t * a.ldg + at])) : y; }
+
+constexpr float kNone = -3e38f; // a maximum of nothing: a number, so that the differences to it are
+
+// the rows of an item and the tiles that they see: [0, n_keep) in kt tiles, then [lo, i1] in tiles from position TILE * w0 on
+struct item {
+    int s, rg, row0, rows; // rows [row0, row0 + rows) of the sequence: its tokens x the query heads of a key head
+    int p0, i0, i1;        // positions of its first token, of the item's first and last
+    int lo, n_keep, kt, w0, n;
+    int64_t t0;            // its first token
+};
+template <int R, int TILE> __device__ __forceinline__ item item_of(const attn_args &a, int s, int rg) {
+    item x;
+    const int hpg = a.H / a.G;
+    x.s = s, x.rg = rg, x.t0 = a.starts[s], x.p0 = a.pos0[s], x.row0 = rg * R;
+    const int64_t all = (a.starts[s + 1] - x.t0) * hpg;
+    x.rows = (int)min((int64_t)R, all - x.row0);
+    x.n = 0;
+    if (x.rows <= 0 || all <= a.rows_above || all > a.rows_up_to) return x;
+    x.i0 = x.p0 + x.row0 / hpg, x.i1 = x.p0 + (x.row0 + x.rows - 1) / hpg;
+    x.lo = a.window > 0 ? (int)max((int64_t)0, x.i0 - a.window + 1) : 0;
+    x.n_keep = (int)min(a.keep, (int64_t)x.lo);
+    x.kt = (x.n_keep + TILE - 1) / TILE, x.w0 = x.lo / TILE;
+    x.n = x.kt + x.i1 / TILE - x.w0 + 1;
+    return x;
+}
+
+// The tiles of a call lie in one row, head by head of every item, each with kBegin units of no work ahead of its tiles (what it costs to begin an item).  CTA b of N has U / N of these units, and one more where b < U % N.
+struct deal {
+    unsigned each, more;
+    __device__ __forceinline__ deal(unsigned U, unsigned N) : each(U / N), more(U - U / N * N) {}
+    __device__ __forceinline__ unsigned first(unsigned b) const { return b * each + min(b, more); }
+    __device__ __forceinline__ unsigned owner(unsigned u) const { return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each; }
+};
+// what a CTA works on at a time: tiles [tile, tile + n) of an item and head
+struct piece {
+    item it;
+    int entry, head, tile, n;
+    unsigned u; // the head's first unit
+};
+// the first piece from unit `at` on, which lies in the head that begins at x.u; n 0: none ahead of `end`
+template <int R, int TILE, int kBegin> __device__ __forceinline__ void piece_from(const attn_args &a, piece &x, unsigned at, unsigned end) {
+    for (;;) {
+        x.tile = max(0, (int)(at - x.u) - kBegin), x.n = (int)min((unsigned)(x.it.n + kBegin), end - x.u) - kBegin - x.tile;
+        if (x.n > 0) return;
+        x.n = 0, x.u += x.it.n + kBegin, at = x.u;
+        if (at >= end) return;
+        if (++x.head == a.G) {
+            x.head = 0;
+            do {
+                x.entry++;
+                x.it = item_of<R, TILE>(a, x.entry / a.groups, x.entry % a.groups);
+            } while (x.it.n == 0);
+        }
+    }
+}
 
 } // namespace kv8
 #endif

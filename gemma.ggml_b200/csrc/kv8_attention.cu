@@ -24,70 +24,16 @@
 #include <cuda.h>
 
 #include "kv8.cuh"
+#include "kv8_tile.cuh"
 
 namespace {
 
 using namespace kv8;
 
 constexpr int kMaxRows = 32, kMaxCtas = 512;
-constexpr float kNone = -3e38f; // a maximum of nothing: a number, so that the differences to it are
+constexpr int kBegin = 2; // units that an item costs to begin: the queries, the warps' sums
 
 inline size_t part_bytes(int Dv) { return (size_t)kMaxCtas * (2 * kMaxRows * (size_t)(Dv + 2) * 4 + 2 * sizeof(int4)); }
-
-// the rows of an item and the tiles that they see: [0, n_keep) in kt tiles, then [lo, i1] in tiles from position TILE * w0 on
-struct item {
-    int s, rg, row0, rows; // rows [row0, row0 + rows) of the sequence: its tokens x the query heads of a key head
-    int p0, i0, i1;        // positions of its first token, of the item's first and last
-    int lo, n_keep, kt, w0, n;
-    int64_t t0;            // its first token
-};
-template <int R, int TILE> __device__ __forceinline__ item item_of(const attn_args &a, int s, int rg) {
-    item x;
-    const int hpg = a.H / a.G;
-    x.s = s, x.rg = rg, x.t0 = a.starts[s], x.p0 = a.pos0[s], x.row0 = rg * R;
-    const int64_t all = (a.starts[s + 1] - x.t0) * hpg;
-    x.rows = (int)min((int64_t)R, all - x.row0);
-    x.n = 0;
-    if (x.rows <= 0) return x;
-    x.i0 = x.p0 + x.row0 / hpg, x.i1 = x.p0 + (x.row0 + x.rows - 1) / hpg;
-    x.lo = a.window > 0 ? (int)max((int64_t)0, x.i0 - a.window + 1) : 0;
-    x.n_keep = (int)min(a.keep, (int64_t)x.lo);
-    x.kt = (x.n_keep + TILE - 1) / TILE, x.w0 = x.lo / TILE;
-    x.n = x.kt + x.i1 / TILE - x.w0 + 1;
-    return x;
-}
-
-// The tiles of a call lie in one row, head by head of every item, each with kBegin units of no work ahead of its tiles (what it costs to begin an item: queries, the warps'
-// sums).  CTA b of N has U / N of these units, and one more where b < U % N.
-constexpr int kBegin = 2;
-struct deal {
-    unsigned each, more;
-    __device__ __forceinline__ deal(unsigned U, unsigned N) : each(U / N), more(U - U / N * N) {}
-    __device__ __forceinline__ unsigned first(unsigned b) const { return b * each + min(b, more); }
-    __device__ __forceinline__ unsigned owner(unsigned u) const { return u < more * (each + 1) ? u / (each + 1) : more + (u - more * (each + 1)) / each; }
-};
-// what a CTA works on at a time: tiles [tile, tile + n) of an item and head
-struct piece {
-    item it;
-    int entry, head, tile, n;
-    unsigned u; // the head's first unit
-};
-// the first piece from unit `at` on, which lies in the head that begins at x.u; n 0: none ahead of `end`
-template <int R, int TILE> __device__ __forceinline__ void piece_from(const attn_args &a, piece &x, unsigned at, unsigned end) {
-    for (;;) {
-        x.tile = max(0, (int)(at - x.u) - kBegin), x.n = (int)min((unsigned)(x.it.n + kBegin), end - x.u) - kBegin - x.tile;
-        if (x.n > 0) return;
-        x.n = 0, x.u += x.it.n + kBegin, at = x.u;
-        if (at >= end) return;
-        if (++x.head == a.G) {
-            x.head = 0;
-            do {
-                x.entry++;
-                x.it = item_of<R, TILE>(a, x.entry / a.groups, x.entry % a.groups);
-            } while (x.it.n == 0);
-        }
-    }
-}
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -284,7 +230,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                 }
             else x.entry = e0;
             x.head = (int)((u - base) / (unsigned)(x.it.n + kBegin)), x.u = base + x.head * (x.it.n + kBegin);
-            piece_from<R, Z::tile>(a, x, u, end);
+            piece_from<R, Z::tile, kBegin>(a, x, u, end);
             s_piece[0] = x, s_end = end, s_all = U;
         }
     } else if (tid == 0) {
@@ -301,7 +247,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
         const unsigned at = x.u + kBegin + x.tile + x.n;
         const bool more = x.n > 0 && at < s_end;
         x.n = 0;
-        if (more) piece_from<R, Z::tile>(a, x, at, s_end);
+        if (more) piece_from<R, Z::tile, kBegin>(a, x, at, s_end);
         s_piece[to] = x;
     };
     auto stage_queries = [&](const piece &x) {
@@ -778,6 +724,30 @@ template <int CODE, int PARTS> int step_rows(const attn_args &a, int64_t max_new
     return rows <= 8 ? step_launch<CODE, 256, 1, PARTS>(a, max_new) : step_launch<CODE, 256, 2, PARTS>(a, max_new);
 }
 
+// sequences of many rows by the tiles' kernel, the others by the steps'
+constexpr int64_t kFew = 32;
+template <int CODE, int PARTS> int attend(attn_args a, int64_t T, int64_t max_new) {
+    using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
+    const int64_t hpg = a.H / a.G;
+    const bool tiles = max_new * hpg > kFew && tile_fits(a.D, a.Dv, a.H, a.G), steps = !tiles || (a.n_seq > 1 && hpg <= kFew);
+    if (steps) {
+        a.rows_above = 0, a.rows_up_to = tiles ? kFew : INT64_MAX;
+        const int rc = step_rows<CODE, PARTS>(a, tiles ? kFew / hpg : max_new);
+        if (rc) return rc;
+    }
+    if (tiles) {
+        a.rows_above = steps ? kFew : 0, a.rows_up_to = INT64_MAX;
+        unsigned joins;
+        const int rc = tile_launch<CODE, PARTS>(a, T, max_new, &joins);
+        if (rc) return rc;
+        if (joins) {
+            GGB_CUDA(ggb_launch_step(kv8_join_kernel<kTileRows, E>, dim3(joins), dim3(256), 0, a));
+            GGB_LAUNCH_CHECK();
+        }
+    }
+    return GGB_OK;
+}
+
 } // namespace
 
 extern "C" {
@@ -802,10 +772,10 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
                   scratch_bytes, part_bytes(Dv));
     float *part = (float *)scratch;
     const attn_args a{q, (const uint8_t *)cache, tables, table_ld, block_size, n_seq, starts, pos0, H, G, D, Dv, window, window > 0 ? keep_first : 0, softcap, sink, gate, ldg,
-                           kv8_record(D, Dv, block_size), out, 0, part, part ? (int4 *)(part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2)) : nullptr,
-                           (uintptr_t)q % 16 == 0, ggb_wait_error_flag()};
-    if (dt == GGB_TYPE_BF16) return code == GGB_KV8_INT8 ? step_rows<GGB_KV8_INT8, 1>(a, max_new) : step_rows<GGB_KV8_E4M3, 1>(a, max_new);
-    return code == GGB_KV8_INT8 ? step_rows<GGB_KV8_INT8, 2>(a, max_new) : step_rows<GGB_KV8_E4M3, 2>(a, max_new);
+                      kv8_record(D, Dv, block_size), out, 0, 0, 0, part, part ? (int4 *)(part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2)) : nullptr, (uintptr_t)q % 16 == 0,
+                      (uintptr_t)out % 16 == 0, ggb_wait_error_flag()};
+    if (dt == GGB_TYPE_BF16) return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 1>(a, T, max_new) : attend<GGB_KV8_E4M3, 1>(a, T, max_new);
+    return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 2>(a, T, max_new) : attend<GGB_KV8_E4M3, 2>(a, T, max_new);
 }
 
 } // extern "C"
