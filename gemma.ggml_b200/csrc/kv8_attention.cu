@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
     }
 }
 
-// an item's pieces, by the CTAs of the same numbers as those that hold them, all but the last: a share of the item's numbers each.  Threads of a column of four numbers have
+// an item's pieces, by the CTAs of the same numbers as those that hold them, all but the last: a share of the item's numbers each (many rows: gridDim.y shares).  Threads of a column of four numbers have
 // the pieces in turn, four of them asked for ahead of the rows' maxima and sums, and are added up in order
 template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_kernel(const __grid_constant__ attn_args a) {
     __shared__ float4 s_y[256];
@@ -623,7 +623,7 @@ template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_ker
     step_wait();
     const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
     if (d.x < 0) return;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hpg = a.H / a.G, b0 = e.x, pieces = e.y - b0 + 1, share = blockIdx.x - b0, shares = pieces - 1;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hpg = a.H / a.G, b0 = e.x, pieces = e.y - b0 + 1, share = (blockIdx.x - b0) * gridDim.y + blockIdx.y, shares = (pieces - 1) * gridDim.y;
     const int64_t pitch = a.Dv + 2;
     const int quads = a.Dv / 4, rows = d.y, q0 = rows * quads * share / shares, q1 = rows * quads * (share + 1) / shares, r0 = q0 / quads;
     if (q0 == q1) return;
@@ -741,7 +741,7 @@ template <int CODE, int PARTS> int attend(attn_args a, int64_t T, int64_t max_ne
         const int rc = tile_launch<CODE, PARTS>(a, T, max_new, &joins);
         if (rc) return rc;
         if (joins) {
-            GGB_CUDA(ggb_launch_step(kv8_join_kernel<kTileRows, E>, dim3(joins), dim3(256), 0, a));
+            GGB_CUDA(ggb_launch_step(kv8_join_kernel<kTileRows, E>, dim3(joins, 8), dim3(256), 0, a));
             GGB_LAUNCH_CHECK();
         }
     }

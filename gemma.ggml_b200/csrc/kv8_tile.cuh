@@ -23,9 +23,14 @@ namespace kv8 {
 
 constexpr int kTileRows = 128, kTileKeys = 64, kTileBegin = 6; // (an item costs about six tiles to begin and to end)
 constexpr int kTileCtas = 128;                                 // that share items: their pieces fill the workspace
-constexpr int kSoftWarps = 16, kCodeWarps = 4, kTileThreads = 32 * (kSoftWarps + kCodeWarps + 1), kTileMma = kSoftWarps + kCodeWarps;
+constexpr int kSoftWarps = 16, kCodeWarps = 4, kTileThreads = 32 * (kSoftWarps + kCodeWarps + 4), kTileMma = kSoftWarps + kCodeWarps;
+// registers: six groups of four warps are launched with 80 a thread, of which the weights' take 96 and the others 64 and 32 (4 x 96 + 64 + 32 = 6 x 80)
+constexpr int kSoftRegs = 96, kCodeRegs = 64, kMmaRegs = 32;
 constexpr int kAhead = 3; // tiles of codes asked for
 enum { T_K_FULL = 0, T_K_FREE = 16, T_V_FULL = 32, T_V_FREE = 48, T_S_FULL = 64, T_P_FULL = 80, T_DONE = 96, T_Q_FULL = 104, T_SLOT = 128, T_DEAD = 132 };
+
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 struct tile_sizes {
     uint32_t q, k, v, raw, raw_stage, stats, scales, bars, smem; // byte offsets behind the 1024-byte boundary, and bytes in all
@@ -45,8 +50,8 @@ struct tile_mma {
     volatile int *dead;
 };
 __device__ __forceinline__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
-// the MMAs of a piece's n tiles: ph, uses of the two stages so far, `pieces` pieces so far
-template <int PARTS> __device__ __forceinline__ void tile_products(const tile_mma &m, int n, int ph0, int ph1, int pieces) {
+// the MMAs of a piece's n tiles: ph, uses of the two stages so far, `pieces` pieces so far.  KS: D / 16, or 0 for a number known at run time only
+template <int PARTS, int KS> __device__ __forceinline__ void tile_products(const tile_mma &m, int n, int ph0, int ph1, int pieces) {
     const uint32_t id_s = idesc_f16(kTileRows, kTileKeys, false), id_o = idesc_f16(kTileRows, m.Dv, true);
     const uint32_t q_lo = umma_desc_lo(m.q, 16), k_lo = umma_desc_lo(m.k, 16), v_lo = umma_desc_lo(m.v, kTileKeys * 128);
     auto scores = [&](int t) {
@@ -54,9 +59,16 @@ template <int PARTS> __device__ __forceinline__ void tile_products(const tile_mm
         mbar_wait_bounded(m.bars + T_K_FULL + 8 * s, par, m.dead);
         tc_fence_after();
 #pragma unroll
-        for (int part = PARTS - 1; part >= 0; part--) // the small part first
-            for (int k = 0; k < m.ksteps; k++)
-                umma_ss(d, q_lo + part * (m.q_part >> 4) + (k >> 2) * (kTileRows * 8) + 2 * (k & 3), kl + (k >> 2) * (kTileKeys * 8) + 2 * (k & 3), id_s, part < PARTS - 1 || k > 0);
+        for (int part = PARTS - 1; part >= 0; part--) { // the small part first
+            const uint32_t ql = q_lo + part * (m.q_part >> 4);
+            if (KS > 0) {
+#pragma unroll
+                for (int k = 0; k < KS; k++) umma_ss(d, ql + (k >> 2) * (kTileRows * 8) + 2 * (k & 3), kl + (k >> 2) * (kTileKeys * 8) + 2 * (k & 3), id_s, part < PARTS - 1 || k > 0);
+            } else {
+                for (int k = 0; k < m.ksteps; k++)
+                    umma_ss(d, ql + (k >> 2) * (kTileRows * 8) + 2 * (k & 3), kl + (k >> 2) * (kTileKeys * 8) + 2 * (k & 3), id_s, part < PARTS - 1 || k > 0);
+            }
+        }
         umma_arrive(m.bars + T_S_FULL + 8 * s);
         umma_arrive(m.bars + T_K_FREE + 8 * s);
     };
@@ -178,106 +190,141 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
     const int D64 = (a.D + 63) / 64, V64 = (a.Dv + 63) / 64;
     const uint32_t q_part = D64 * kTileRows * 128, k_stage = D64 * kTileKeys * 128, v_stage = V64 * kTileKeys * 128;
 
-    int ph0 = 0, ph1 = 0, pieces = 0; // uses of the two stages, pieces so far
-    for (int slot = 0; s_piece[slot].n > 0; slot ^= 1, pieces++) {
-        const piece &x = s_piece[slot];
-        const item &it = x.it;
-        const int n = x.n, tile = x.tile;
-        auto first_of = [&](int t) { return (t < it.kt ? t : it.w0 + t - it.kt) * kTileKeys; };
-        if (warp >= kSoftWarps && warp < kTileMma) {
-            // ---- codes: this warp's 16 positions of every tile.  A lane takes rows (lane >> 2) and 8 on, 16 codes of every 64
-            const int cw = warp - kSoftWarps, r0 = lane >> 2, c = 16 * (lane & 3);
-            const uint32_t ring = base + z.raw + cw * kAhead * z.raw_stage + 16 * lane;
+    // the roles, each through all pieces; ph0, ph1: uses of the two stages so far
+    auto next_piece = [&] { // all threads: what a piece was is no longer needed
+        tc_fence_before();
+        warp_meet();
+        bar_sync(0, kTileThreads);
+        tc_fence_after();
+    };
+    int ph0 = 0, ph1 = 0;
+    if (warp >= kSoftWarps && warp < kTileMma) {
+        // ---- codes: a warp has 16 positions of every tile, a lane rows (lane >> 2) and 8 on, 16 codes of every 64
+        fewer_registers<kCodeRegs>();
+        const int cw = warp - kSoftWarps, r0 = lane >> 2, c = 16 * (lane & 3);
+        const uint32_t ring = base + z.raw + cw * kAhead * z.raw_stage + 16 * lane, scale_at = base + z.scales + 8 * cw + 4 * lane; // (lanes 0 and 1: keys', values')
+        const int r = 16 * cw + r0, pc = 2 * (lane & 3); // rows r and r + 8 of a tile: the same place within 8 rows
+        const uint32_t at0 = r * 128 + ((pc ^ (r & 7)) << 4), at1 = r * 128 + (((pc + 1) ^ (r & 7)) << 4);
+        int stage = 0;
+        for (int slot = 0; s_piece[slot].n > 0; slot ^= 1) {
+            const item &it = s_piece[slot].it;
+            const int n = s_piece[slot].n, tile = s_piece[slot].tile, head = s_piece[slot].head;
+            const int kt = it.kt, w0 = it.w0 - kt, n_keep = it.n_keep, lo = it.lo, i1 = it.i1;
             const int32_t *table = a.tables + it.s * a.table_ld;
-            auto seen = [&](int t, int first) { return t < it.kt ? first < it.n_keep : first + 15 >= it.lo && first <= it.i1; };
+            auto first_of = [&](int k) { return (tile + k < kt ? tile + k : w0 + tile + k) * kTileKeys + 16 * cw; };
+            auto seen = [&](int k, int first) { return tile + k < kt ? first < n_keep : first + 15 >= lo && first <= i1; };
             int page = -1; // of the group that is asked for next
             auto look = [&](int k) {
-                const int first = first_of(tile + k) + 16 * cw;
-                page = k < n && seen(tile + k, first) ? table[first / a.B] : -1;
+                const int first = first_of(k);
+                page = k < n && seen(k, first) ? table[first / a.B] : -1;
             };
-            float2 sc[kAhead];
-            auto ask = [&](int k, int stage, float2 &scale) {
-                scale = make_float2(0.f, 0.f);
+            auto ask = [&](int k, int to_stage) {
+                const uint32_t to_scale = scale_at + ((ph0 + ph1 + k) & 7) * 32;
                 if (page >= 0) {
-                    const int row = (first_of(tile + k) + 16 * cw) % a.B;
-                    const uint8_t *rec = a.cache + ((int64_t)page * a.G + x.head) * a.record, *kp = rec + row * a.D + c, *vp = rec + a.B * a.D + row * a.Dv + c;
-                    const float *sp = reinterpret_cast<const float *>(rec + a.B * (a.D + a.Dv)) + row / kKv8Group;
-                    const uint32_t to = ring + stage * z.raw_stage;
-                    for (int b = 0; b < D64; b++)
+                    const int row = first_of(k) % a.B;
+                    const uint8_t *rec = a.cache + ((int64_t)page * a.G + head) * a.record, *kp = rec + (row + r0) * a.D + c, *vp = rec + a.B * a.D + (row + r0) * a.Dv + c;
+                    const uint32_t to = ring + to_stage * z.raw_stage;
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
                         if (64 * b + c < a.D) {
-                            cp_async16(to + b * 1024, kp + r0 * a.D + 64 * b);
-                            cp_async16(to + b * 1024 + 512, kp + (r0 + 8) * a.D + 64 * b);
+                            cp_async16(to + b * 1024, kp + 64 * b);
+                            cp_async16(to + b * 1024 + 512, kp + 8 * a.D + 64 * b);
                         }
-                    for (int b = 0; b < V64; b++)
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
                         if (64 * b + c < a.Dv) {
-                            cp_async16(to + (D64 + b) * 1024, vp + r0 * a.Dv + 64 * b);
-                            cp_async16(to + (D64 + b) * 1024 + 512, vp + (r0 + 8) * a.Dv + 64 * b);
+                            cp_async16(to + (D64 + b) * 1024, vp + 64 * b);
+                            cp_async16(to + (D64 + b) * 1024 + 512, vp + 8 * a.Dv + 64 * b);
                         }
-                    scale = make_float2(sp[0], sp[a.B / kKv8Group]);
+                    if (lane < 2) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to_scale), "l"(rec + a.B * (a.D + a.Dv) + (row + lane * a.B) / 4) : "memory");
+                } else if (k < n && lane < 2) {
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(to_scale), "r"(0) : "memory");
                 }
                 cp_async_commit();
                 look(k + 1);
             };
-            look(0);
-            for (int k = 0; k < kAhead - 1; k++) ask(k, k, sc[k]);
-            int stage = 0;
-            for (int k = 0; k < n; k++) {
-                const int s = k & 1, uses = (s ? ph1 : ph0) + (k >> 1), first = first_of(tile + k) + 16 * cw;
-                float2 ahead;
-                ask(k + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1, ahead);
-                cp_async_wait<kAhead - 1>();
-                const bool here = seen(tile + k, first);
-                // 16 codes of row r0 (+ 8) to two places of a row of 128 bytes, swizzled
-                auto lay_out = [&](uint32_t from, uint32_t to, int blocks, int width, bool zero_behind) {
-                    for (int b = 0; b < blocks; b++)
+            // a lane's codes of keys, or of values, to their places
+            auto lay_out = [&](uint32_t from, uint32_t to, int blocks, int width, bool zero0, bool zero1) {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    if (b < blocks) {
+                        uint4 w[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[e].x), "=r"(w[e].y), "=r"(w[e].z), "=r"(w[e].w) : "r"(from + b * 1024 + e * 512) : "memory");
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             uint32_t h[8];
-                            uint4 w;
-                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(from + b * 1024 + e * 512) : "memory");
-                            halves_of<CODE>(w.x, h[0], h[1]);
-                            halves_of<CODE>(w.y, h[2], h[3]);
-                            halves_of<CODE>(w.z, h[4], h[5]);
-                            halves_of<CODE>(w.w, h[6], h[7]);
-                            // behind the end of a row zeros, and behind the last position, where codes may be no numbers, which a weight of zero would not undo
-                            if (64 * b + c >= width || (zero_behind && (!here || first + r0 + 8 * e > it.i1)))
+                            halves_of<CODE>(w[e].x, h[0], h[1]);
+                            halves_of<CODE>(w[e].y, h[2], h[3]);
+                            halves_of<CODE>(w[e].z, h[4], h[5]);
+                            halves_of<CODE>(w[e].w, h[6], h[7]);
+                            if (64 * b + c >= width || (e ? zero1 : zero0))
 #pragma unroll
                                 for (int u = 0; u < 8; u++) h[u] = 0;
-                            const int r = 16 * cw + r0 + 8 * e;
-                            const uint32_t row = to + b * (kTileKeys * 128) + r * 128, pc = 2 * (lane & 3);
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((pc ^ (r & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + (((pc + 1) ^ (r & 7)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                            const uint32_t row = to + b * (kTileKeys * 128) + e * 1024;
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + at0), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + at1), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                         }
-                    fence_async_smem();
-                    __syncwarp();
-                };
+                    }
+                fence_async_smem();
+                __syncwarp();
+            };
+            look(0);
+            for (int k = 0, s = stage; k < kAhead - 1; k++) {
+                ask(k, s);
+                if (++s == kAhead) s = 0;
+            }
+            for (int k = 0; k < n; k++) {
+                const int s = k & 1, uses = (s ? ph1 : ph0) + (k >> 1), first = first_of(k);
+                ask(k + kAhead - 1, stage == 0 ? kAhead - 1 : stage - 1);
+                cp_async_wait<kAhead - 1>();
                 const uint32_t from = ring + stage * z.raw_stage;
                 if (uses > 0 && !mbar_wait_warp(bars + T_K_FREE + 8 * s, (uses - 1) & 1, dead)) break;
-                lay_out(from, base + z.k + s * k_stage, D64, a.D, false);
-                if (lane == 0) {
-                    scales[((ph0 + ph1 + k) & 7) * 4 + cw] = sc[0];
-                    mbar_arrive(bars + T_K_FULL + 8 * s);
-                }
+                lay_out(from, base + z.k + s * k_stage, D64, a.D, false, false);
+                if (lane == 0) mbar_arrive(bars + T_K_FULL + 8 * s);
                 if (uses > 0 && !mbar_wait_warp(bars + T_V_FREE + 8 * s, (uses - 1) & 1, dead)) break;
-                lay_out(from + D64 * 1024, base + z.v + s * v_stage, V64, a.Dv, true);
+                // behind the last position, and where nothing was asked for, there may be codes that are no numbers, which a weight of zero would not undo
+                const bool none = !seen(k, first);
+                lay_out(from + D64 * 1024, base + z.v + s * v_stage, V64, a.Dv, none || first + r0 > i1, none || first + r0 + 8 > i1);
                 if (lane == 0) mbar_arrive(bars + T_V_FULL + 8 * s);
                 if (++stage == kAhead) stage = 0;
-#pragma unroll
-                for (int u = 0; u < kAhead - 2; u++) sc[u] = sc[u + 1];
-                sc[kAhead - 2] = ahead;
             }
             cp_async_wait<0>();
-        } else if (warp == kTileMma) {
-            const tile_mma m{bars, base + z.q, q_part, base + z.k, k_stage, base + z.v, v_stage, tmem, (a.D + 15) / 16, a.Dv, dead};
-            tile_products<PARTS>(m, n, ph0, ph1, pieces);
-        } else {
+            ph0 += (n + 1) / 2, ph1 += n / 2;
+            next_piece();
+        }
+    } else if (warp >= kTileMma) {
+        // ---- products, by the first of these warps
+        fewer_registers<kMmaRegs>();
+        int pieces = 0;
+        for (int slot = 0; s_piece[slot].n > 0; slot ^= 1, pieces++) {
+            const int n = s_piece[slot].n;
+            if (warp == kTileMma) {
+                const tile_mma m{bars, base + z.q, q_part, base + z.k, k_stage, base + z.v, v_stage, tmem, a.D / 16, a.Dv, dead};
+                if (a.D == 128) tile_products<PARTS, 8>(m, n, ph0, ph1, pieces);
+                else if (a.D == 64) tile_products<PARTS, 4>(m, n, ph0, ph1, pieces);
+                else tile_products<PARTS, 0>(m, n, ph0, ph1, pieces);
+            }
+            ph0 += (n + 1) / 2, ph1 += n / 2;
+            next_piece();
+        }
+    } else {
+        more_registers<kSoftRegs>();
+        int pieces = 0;
+        for (int slot = 0; s_piece[slot].n > 0; slot ^= 1, pieces++) {
+            const piece &x = s_piece[slot];
+            const item &it = x.it;
+            const int n = x.n, tile = x.tile;
+            auto first_of = [&](int t) { return (t < it.kt ? t : it.w0 + t - it.kt) * kTileKeys; };
             // ---- queries: a warp's 8 rows
             float *srow = st + 12 * kTileRows;
-            {
-                float4 v[8];
+#pragma unroll 1
+            for (int u0 = 0; u0 < 8; u0 += 4) {
+                float4 v[4];
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    const int r = 8 * warp + u, row = it.row0 + r, tq = row / hpg, h = x.head * hpg + (row - tq * hpg);
+                for (int u = 0; u < 4; u++) {
+                    const int r = 8 * warp + u0 + u, row = it.row0 + r, tq = row / hpg, h = x.head * hpg + (row - tq * hpg);
                     v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (r < it.rows && 4 * lane < a.D) {
                         const float *src = a.q + ((it.t0 + tq) * a.H + h) * a.D + 4 * lane;
@@ -286,8 +333,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                     }
                 }
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    const int r = 8 * warp + u;
+                for (int u = 0; u < 4; u++) {
+                    const int r = 8 * warp + u0 + u;
                     const float big = fmaxf(fmaxf(fabsf(v[u].x), fabsf(v[u].y)), fmaxf(fabsf(v[u].z), fabsf(v[u].w))), most = warp_max_f32(big);
                     const bool odd = __any_sync(0xffffffffu, big == INFINITY || v[u].x != v[u].x || v[u].y != v[u].y || v[u].z != v[u].z || v[u].w != v[u].w);
                     const float f = odd ? 0.f : power_for(most, 10);
@@ -454,12 +501,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                 a.desc[2 * blockIdx.x] = make_int4(it.s, it.rows, x.head, it.row0);
                 a.desc[2 * blockIdx.x + 1] = make_int4((int)d.owner(x.u + kTileBegin), (int)d.owner(x.u + kTileBegin + it.n - 1), (int)it.t0, 0);
             }
-            tc_fence_before();
+            ph0 += (n + 1) / 2, ph1 += n / 2;
+            next_piece();
         }
-        ph0 += (n + 1) / 2, ph1 += n / 2;
-        warp_meet();
-        __syncthreads();
-        tc_fence_after();
     }
     warp_meet();
     __syncthreads();
@@ -482,6 +526,11 @@ template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t m
     auto kfn = kv8_tile_kernel<CODE, PARTS>;
     const int rc = ggb_allow_smem(kfn, smem);
     if (rc) return rc;
+    static const int registers = [kfn] { // what the split takes has to be there, or it would be waited for without end
+        cudaFuncAttributes at{};
+        return cudaFuncGetAttributes(&at, kfn) == cudaSuccess ? at.numRegs : 0;
+    }();
+    GGB_CHECK_ARG(registers * (kTileThreads / 128) >= 4 * kSoftRegs + kCodeRegs + kMmaRegs, "kv8_attn: built with %d registers a thread", registers);
     const unsigned ctas = (unsigned)(a.part ? std::min(kTileCtas, ggb_sm_count()) : ggb_sm_count());
     GGB_CUDA(ggb_launch_early(kfn, ggb_cluster{1, 1, 1}, dim3(ctas), dim3(kTileThreads), smem, a));
     GGB_LAUNCH_CHECK();
