@@ -63,7 +63,7 @@ template <int PARTS, int KS> __device__ __forceinline__ void tile_products(const
             const uint32_t ql = q_lo + part * (m.q_part >> 4);
             if (KS > 0) {
 #pragma unroll
-                for (int k = 0; k < KS; k++) umma_ss(d, ql + (k >> 2) * (kTileRows * 8) + 2 * (k & 3), kl + (k >> 2) * (kTileKeys * 8) + 2 * (k & 3), id_s, part < PARTS - 1 || k > 0);
+                for (int b = 0; b < KS / 4; b++) umma_ss_k4(d, ql + b * (kTileRows * 8), kl + b * (kTileKeys * 8), id_s, part < PARTS - 1 || b > 0);
             } else {
                 for (int k = 0; k < m.ksteps; k++)
                     umma_ss(d, ql + (k >> 2) * (kTileRows * 8) + 2 * (k & 3), kl + (k >> 2) * (kTileKeys * 8) + 2 * (k & 3), id_s, part < PARTS - 1 || k > 0);
@@ -82,9 +82,7 @@ template <int PARTS, int KS> __device__ __forceinline__ void tile_products(const
         tc_fence_after();
         const uint32_t o = m.tmem + 128 + s * m.Dv, p = m.tmem + s * 64, vl = v_lo + ((s * m.v_stage) >> 4);
 #pragma unroll
-        for (int part = PARTS - 1; part >= 0; part--)
-#pragma unroll
-            for (int k = 0; k < kTileKeys / 16; k++) umma_ts(o, p + part * 32 + 8 * k, vl + k * 128, id_o, part < PARTS - 1 || k > 0 ? 1u : t >= 2);
+        for (int part = PARTS - 1; part >= 0; part--) umma_ts_k4(o, p + part * 32, vl, 128, id_o, part < PARTS - 1 ? 1u : t >= 2);
         umma_arrive(m.bars + T_V_FREE + 8 * s);
         if (t + 2 < n) scores(t + 2);
     }
@@ -205,6 +203,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
         const uint32_t ring = base + z.raw + cw * kAhead * z.raw_stage + 16 * lane, scale_at = base + z.scales + 8 * cw + 4 * lane; // (lanes 0 and 1: keys', values')
         const int r = 16 * cw + r0, pc = 2 * (lane & 3); // rows r and r + 8 of a tile: the same place within 8 rows
         const uint32_t at0 = r * 128 + ((pc ^ (r & 7)) << 4), at1 = r * 128 + (((pc + 1) ^ (r & 7)) << 4);
+        const int per_pages = kTileKeys / a.B, per_rows = kTileKeys - per_pages * a.B;
         int stage = 0;
         for (int slot = 0; s_piece[slot].n > 0; slot ^= 1) {
             const item &it = s_piece[slot].it;
@@ -213,15 +212,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
             const int32_t *table = a.tables + it.s * a.table_ld;
             auto first_of = [&](int k) { return (tile + k < kt ? tile + k : w0 + tile + k) * kTileKeys + 16 * cw; };
             auto seen = [&](int k, int first) { return tile + k < kt ? first < n_keep : first + 15 >= lo && first <= i1; };
-            int page = -1; // of the group that is asked for next
+            // the group that is asked for next: its page, or -1, and row.  From a tile to the next the place in the table and the row move by what a tile is in pages and rows
+            int page = -1, at_page = 0, at_row = 0;
             auto look = [&](int k) {
                 const int first = first_of(k);
-                page = k < n && seen(k, first) ? table[first / a.B] : -1;
+                if (k == 0 || tile + k == kt) {
+                    at_page = first / a.B, at_row = first - at_page * a.B;
+                } else {
+                    at_page += per_pages, at_row += per_rows;
+                    if (at_row >= a.B) at_row -= a.B, at_page++;
+                }
+                page = -1;
+                if (k < n && seen(k, first)) page = table[at_page];
             };
             auto ask = [&](int k, int to_stage) {
                 const uint32_t to_scale = scale_at + ((ph0 + ph1 + k) & 7) * 32;
                 if (page >= 0) {
-                    const int row = first_of(k) % a.B;
+                    const int row = at_row;
                     const uint8_t *rec = a.cache + ((int64_t)page * a.G + head) * a.record, *kp = rec + (row + r0) * a.D + c, *vp = rec + a.B * a.D + (row + r0) * a.Dv + c;
                     const uint32_t to = ring + to_stage * z.raw_stage;
 #pragma unroll
@@ -369,7 +376,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
             const int lo_last = a.window > 0 ? (int)max((int64_t)0, it.i1 - a.window + 1) : 0;
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + lanes + grp * 64, to = tmem + lanes + 128 + grp * a.Dv;
             const float rowf = srow[r], cap = a.cap * kLog2e, inv_cap = a.cap > 0.f ? kLn2 / a.cap : 0.f;
-            float m = kNone, l = 0.f, vref = 0.f;
+            float m = kNone, l = 0.f, vref = 0.f, vinv = 0.f;
             bool lost = false;
             for (int k = grp; k < n; k += 2) {
                 const int t = tile + k, j0 = first_of(t);
@@ -409,7 +416,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                 const bool more = most_v > 64.f * vref;
                 if (more) {
                     f *= vref / most_v;
-                    vref = most_v;
+                    vref = most_v, vinv = 1.f / most_v;
                 }
                 if (k >= 2 && __any_sync(0xffffffffu, f != 1.f)) { // (its MMAs precede this tile's scores)
 #pragma unroll 1
@@ -422,7 +429,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                     }
                 }
                 f32x2 sum[2] = {0, 0};
-                const float vinv = vref > 0.f ? 1.f / vref : 0.f;
 #pragma unroll
                 for (int g = 0; g < 2; g++) {
                     const float rel = sc[2 * half + g].y * vinv;

@@ -108,6 +108,16 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32
                  "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kUmmaDescHi)
                  : "memory");
 }
+// Four steps of 16 along K under one election: 8 columns of A further each, 16 rows of an MN-major B (b_step descriptor units)
+__device__ __forceinline__ void umma_ts_k4(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t b_step, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p, q, e;\n.reg .b64 b, s;\n.reg .b32 a;\n" GGB_ELECT "setp.ne.b32 p, %4, 0;\nsetp.eq.b32 q, %4, %4;\nmov.b64 b, {%2, %5};\ncvt.u64.u32 s, %6;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\nadd.s64 b, b, s;\nadd.u32 a, %1, 8;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\nadd.s64 b, b, s;\nadd.u32 a, a, 8;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\nadd.s64 b, b, s;\nadd.u32 a, a, 8;\n"
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, q;\n}\n" ::"r"(tmem_d),
+                 "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "n"(kUmmaDescHi), "r"(b_step)
+                 : "memory");
+}
 __device__ __forceinline__ void umma_arrive(uint32_t bar) { // arrives when all MMAs issued so far are done
     asm volatile("{\n.reg .pred e;\n" GGB_ELECT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar) : "memory");
 }
