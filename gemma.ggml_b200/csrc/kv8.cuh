@@ -5,6 +5,7 @@
 // group: 16 consecutive positions of one head, keys and values apart.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <stdint.h>
@@ -69,7 +70,7 @@ struct attn_args {
     int64_t rows_above, rows_up_to; // sequences of more rows (tokens x query heads of a key head) than the one, up to the other, are this kernel's
     float *part;    // [CTA][2][rows][Dv + 2], or null: an item a CTA
     int4 *desc;     // [CTA][2], of an item that begins or goes on here and ends elsewhere: sequence (or -1), rows, key head, first row; first and last CTA that have it, first token
-    int vec_q, vec_out; // queries, results begin on a 16-byte boundary
+    int vec_q, vec_out, vec_gate; // queries, results, rows of the gate begin on a 16-byte boundary
     int *wait_error;
 };
 // four codes as two pairs of fp16 numbers.  int8: code + 128 behind the bits of 1024, less 1152
@@ -162,6 +163,32 @@ template <int R, int TILE, int kBegin> __device__ __forceinline__ void piece_fro
             } while (x.it.n == 0);
         }
     }
+}
+
+__device__ __forceinline__ uint4 lds_u4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds_u2(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+// the cache as lines of 128 bytes (a record is whole lines, and 16 rows of it are): boxes of a group's keys and of its values, piece c of line l of a box at place
+// c ^ (l & 7), so that a quarter of a warp reads pieces of several rows from different banks
+struct line_maps {
+    CUtensorMap k, v;
+};
+__device__ __forceinline__ void request(const line_maps &m, uint32_t k_dst, uint32_t v_dst, int k_line, int v_line, uint32_t bytes, uint32_t bar) { // one lane
+    mbar_expect_tx(bar, bytes);
+    tma_load_2d(k_dst, &m.k, 0, k_line, bar);
+    tma_load_2d(v_dst, &m.v, 0, v_line, bar);
+}
+__device__ __forceinline__ uint32_t in_box(int byte) { return (uint32_t)(byte & ~127) + ((((byte >> 4) & 7) ^ ((byte >> 7) & 7)) << 4) + (byte & 15); }
+inline int make_line_maps(const attn_args &a, line_maps &m) { // (as many lines as a coordinate reaches: where the pool ends is the page tables' matter)
+    const int rc = ggb_tensor_map_bf16(&m.k, a.cache, (1ll << 31) - 1, 64, 64, a.D / 8);
+    return rc ? rc : ggb_tensor_map_bf16(&m.v, a.cache, (1ll << 31) - 1, 64, 64, a.Dv / 8);
 }
 
 } // namespace kv8

@@ -21,8 +21,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#include <cuda.h>
-
 #include "kv8.cuh"
 #include "kv8_tile.cuh"
 
@@ -61,28 +59,6 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint4 lds_u4(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint2 lds_u2(uint32_t at) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-    return v;
-}
-// the cache as lines of 128 bytes (a record is whole lines, and 16 rows of it are): boxes of a group's keys and of its values, piece c of line l of a box at place
-// c ^ (l & 7), so that a quarter of a warp reads pieces of several rows from different banks
-struct line_maps {
-    CUtensorMap k, v;
-};
-__device__ __forceinline__ void request(const line_maps &m, uint32_t k_dst, uint32_t v_dst, int k_line, int v_line, uint32_t bytes, uint32_t bar) { // one lane
-    mbar_expect_tx(bar, bytes);
-    tma_load_2d(k_dst, &m.k, 0, k_line, bar);
-    tma_load_2d(v_dst, &m.v, 0, v_line, bar);
-}
-__device__ __forceinline__ uint32_t in_box(int byte) { return (uint32_t)(byte & ~127) + ((((byte >> 4) & 7) ^ ((byte >> 7) & 7)) << 4) + (byte & 15); }
-
 // P: numbers of a key and of a value, at most: 64, 128 or 256
 template <int CODE, int P, int NT, int PARTS> struct step_sizes {
     static constexpr int R = 8 * NT, KS = P / 16; // blocks of 16 value coordinates
@@ -704,8 +680,7 @@ template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64
     if (rc) return rc;
     const unsigned ctas = a.part ? (unsigned)std::min(kMaxCtas, ggb_sm_count() * Z::min_ctas) : (unsigned)(a.n_seq * a.groups * a.G);
     line_maps maps;
-    rc = ggb_tensor_map_bf16(&maps.k, a.cache, (1ll << 31) - 1, 64, 64, a.D / 8);
-    if (!rc) rc = ggb_tensor_map_bf16(&maps.v, a.cache, (1ll << 31) - 1, 64, 64, a.Dv / 8);
+    rc = make_line_maps(a, maps);
     if (rc) return rc;
     GGB_CUDA(ggb_launch_step(k, dim3(ctas), dim3(Z::threads), Z::smem, a, maps));
     GGB_LAUNCH_CHECK();
@@ -773,7 +748,7 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
     float *part = (float *)scratch;
     const attn_args a{q, (const uint8_t *)cache, tables, table_ld, block_size, n_seq, starts, pos0, H, G, D, Dv, window, window > 0 ? keep_first : 0, softcap, sink, gate, ldg,
                       kv8_record(D, Dv, block_size), out, 0, 0, 0, part, part ? (int4 *)(part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2)) : nullptr, (uintptr_t)q % 16 == 0,
-                      (uintptr_t)out % 16 == 0, ggb_wait_error_flag()};
+                      (uintptr_t)out % 16 == 0, (uintptr_t)gate % 16 == 0 && ldg % 4 == 0, ggb_wait_error_flag()};
     if (dt == GGB_TYPE_BF16) return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 1>(a, T, max_new) : attend<GGB_KV8_E4M3, 1>(a, T, max_new);
     return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 2>(a, T, max_new) : attend<GGB_KV8_E4M3, 2>(a, T, max_new);
 }
