@@ -9,7 +9,7 @@
 //
 //   stats   a CTA a piece of a row: its maximum, the first place of it, and sum of exp(l / temperature - maximum); a sequence's last draft row is not read
 //   pick    a CTA a piece of the row that is drawn from: joins the rows' pieces, decides what stands, sums its piece of the weights; the CTA that is done last finds
-//           the token: the piece by the pieces' sums in order, then the place in it
+//           the token: the piece by the pieces' sums in order, the part of it by its warps', then the place in that
 //
 // Exponentials in fp32 and sums of four of them; beyond that, sums, and the probabilities that judge a draft, in 64 bits.  A weight p - q is a 32-bit difference of
 // 32-bit products: as far off as its exponentials are, and nothing where p and q are the same numbers.  So a decision is another one than in 64 bits throughout only
@@ -22,7 +22,7 @@
 
 namespace {
 
-constexpr int kMaxPieces = 128, kThreads = 256;
+constexpr int kMaxPieces = 64, kThreads = 256, kWarps = kThreads / 32;
 
 struct piece_stats {
     float m;    // maximum
@@ -36,11 +36,11 @@ struct verify_args {
     int n_seq, pieces;
     const int32_t *starts, *drafted;
     const float *u;
-    float inv; // 1 / temperature
-    double inv64;
+    float inv; // log2(e) / temperature
+    double inv64; // 1 / temperature
     int32_t *tokens, *accepted;
     piece_stats *stats; // [R][2][pieces]: target, draft
-    double *sums;       // [n_seq][pieces]
+    double *sums;       // [n_seq][pieces][warps]
     unsigned *done;     // [n_seq]
     int vec_t, vec_d;
 };
@@ -61,19 +61,27 @@ __device__ __forceinline__ int sequence_of(const int32_t *starts, int n_seq, int
 __device__ __forceinline__ bool ahead(float m, int at, float m2, int at2) { return m > m2 || (m == m2 && at < at2); }
 
 constexpr int kPasses = 8, kBlock = 4 * kThreads * kPasses; // 16-byte pieces in flight a thread; numbers in those of a CTA
-__device__ __forceinline__ float4 load4(const float *row, int64_t v, int64_t end, bool vec) {
-    if (vec && v + 4 <= end) return *reinterpret_cast<const float4 *>(row + v);
-    float x[4];
+// numbers i .. i + 3 of n
+__device__ __forceinline__ float4 load4(const float *x, int i, int n, bool vec) {
+    if (vec && i + 4 <= n) return *reinterpret_cast<const float4 *>(x + i);
+    float y[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = v + e < end ? row[v + e] : -INFINITY;
-    return make_float4(x[0], x[1], x[2], x[3]);
+    for (int e = 0; e < 4; e++) y[e] = i + e < n ? x[i + e] : -INFINITY;
+    return make_float4(y[0], y[1], y[2], y[3]);
+}
+// exp((x - m) / temperature) as a power of two, c = log2(e) / temperature: the unit's 2^-22 and the argument's roundings of 2^-24 of itself.  Above expf that saves its
+// steps for large arguments, five of the ten instructions a number; below 2^-126 it is zero.
+__device__ __forceinline__ float power(float x, float m, float c) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - m) * c));
+    return y;
 }
 
 // Each block of numbers waits in registers until the CTA's threads have their common maximum, so that a number costs one exponential and sums are scaled once a block
-template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_stats_kernel(const __grid_constant__ verify_args a) {
-    __shared__ float s_m[2][kThreads / 32];
-    __shared__ int s_at[kThreads / 32];
-    __shared__ double s_s[kThreads / 32];
+template <bool GREEDY> __global__ void __launch_bounds__(kThreads, 5) verify_stats_kernel(const __grid_constant__ verify_args a) {
+    __shared__ float s_m[2][kWarps];
+    __shared__ int s_at[kWarps];
+    __shared__ double s_s[kWarps];
     step_wait();
     const int64_t r = blockIdx.y;
     const int side = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -83,7 +91,7 @@ template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_stats_
     if (side == 1 && r == a.starts[seq + 1] - 1) return; // nothing is judged by it
     const float *row = side ? a.draft + r * a.ld_d : a.target + r * a.ld_t;
     const bool vec = side ? a.vec_d : a.vec_t;
-    const int64_t v0 = blockIdx.x * a.piece, v1 = min(a.V, v0 + a.piece); // pieces are multiples of 4
+    const int64_t v0 = blockIdx.x * a.piece, v1 = min(a.V, v0 + a.piece); // pieces are multiples of 32
     float m = -INFINITY;
     int at = 0x7fffffff;
     double s = 0.0;
@@ -91,9 +99,10 @@ template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_stats_
     int turn = 0;
     for (int64_t b = v0; b < v1; b += kBlock, turn ^= 1) {
         float4 x[kPasses];
+        const int n = (int)min((int64_t)kBlock, v1 - b);
 #pragma unroll
         for (int p = 0; p < kPasses; p++)
-            x[p] = b + 4 * kThreads * p < v1 ? load4(row, b + 4 * kThreads * p + 4 * tid, v1, vec) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            x[p] = 4 * kThreads * p < n ? load4(row + b, 4 * kThreads * p + 4 * tid, n, vec) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         float best = m;
 #pragma unroll
         for (int p = 0; p < kPasses; p++) {
@@ -113,14 +122,13 @@ template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_stats_
             if (lane == 0) s_m[turn][warp] = best; // (two of them in turn: the next block's are written before the last warp has read these)
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < kThreads / 32; w++) best = fmaxf(best, s_m[turn][w]);
-            if (best > m) s *= (double)expf((m - best) * a.inv); // m = -inf: 0
+            for (int w = 0; w < kWarps; w++) best = fmaxf(best, s_m[turn][w]);
+            if (best > m) s *= (double)power(m, best, a.inv); // m = -inf: 0
+            const float top = best == -INFINITY ? 0.f : best; // (numbers of -inf are nothing then too)
 #pragma unroll
             for (int p = 0; p < kPasses; p++)
-                if (b + 4 * kThreads * p < v1) {
-                    auto power = [&](float y) { return y == -INFINITY ? 0.f : expf((y - best) * a.inv); }; // inf and NaN leave NaN
-                    s += (double)((power(x[p].x) + power(x[p].y)) + (power(x[p].z) + power(x[p].w)));
-                }
+                if (4 * kThreads * p < n) // inf and NaN leave NaN
+                    s += (double)((power(x[p].x, top, a.inv) + power(x[p].y, top, a.inv)) + (power(x[p].z, top, a.inv) + power(x[p].w, top, a.inv)));
         }
         m = best;
     }
@@ -140,7 +148,7 @@ template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_stats_
     if (lane == 0) s_s[warp] = s;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < kThreads / 32; w++) {
+        for (int w = 1; w < kWarps; w++) {
             s += s_s[w];
             if (GREEDY && ahead(s_m[0][w], s_at[w], m, at)) m = s_m[0][w], at = s_at[w];
         }
@@ -156,27 +164,26 @@ struct row_stats {
 // a row's pieces, joined by a warp: every lane the answer
 template <bool GREEDY> __device__ __forceinline__ row_stats joined(const piece_stats *p, int pieces, double inv) {
     const int lane = threadIdx.x & 31;
-    piece_stats x[kMaxPieces / 32];
     float m = -INFINITY;
     int at = 0x7fffffff;
     double s = 0.0;
-#pragma unroll
-    for (int u = 0; u < kMaxPieces / 32; u++) {
-        x[u] = lane + 32 * u < pieces ? p[lane + 32 * u] : piece_stats{-INFINITY, 0x7fffffff, 0.0};
-        if (ahead(x[u].m, x[u].at, m, at)) at = x[u].at;
-        m = fmaxf(m, x[u].m);
+#pragma unroll 1
+    for (int c = lane; c < pieces; c += 32) {
+        const piece_stats x = p[c];
+        if (x.m == m || GREEDY) s += x.s;
+        else if (x.m > m) s = x.s + (s > 0.0 ? s * exp(((double)m - (double)x.m) * inv) : s);
+        else s += x.s * exp(((double)x.m - (double)m) * inv); // of a piece of no numbers: NaN times 0
+        if (ahead(x.m, x.at, m, at)) m = x.m, at = x.at;
     }
+    float best = m;
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, off);
+        const float m2 = __shfl_xor_sync(0xffffffffu, best, off);
         const int at2 = __shfl_xor_sync(0xffffffffu, at, off);
-        if (ahead(m2, at2, m, at)) at = at2;
-        m = fmaxf(m, m2);
+        if (ahead(m2, at2, best, at)) best = m2, at = at2;
     }
-#pragma unroll
-    for (int u = 0; u < kMaxPieces / 32; u++)
-        if (32 * u < pieces) s += GREEDY || x[u].m == m ? x[u].s : x[u].s * exp(((double)x[u].m - (double)m) * inv); // of a piece of no numbers: NaN times 0
-    return {m, at, warp_sum_f64(s)};
+    if (!GREEDY && m != best) s = s * exp(((double)m - (double)best) * inv);
+    return {best, at, warp_sum_f64(s)};
 }
 
 // the row that the token behind the draft is drawn from
@@ -187,31 +194,14 @@ struct drawn_row {
     int64_t without; // a token that falls out, or -1
 };
 __device__ __forceinline__ float weight(const drawn_row &d, float inv, float lp, float lq, int64_t v) {
-    float w = lp == -INFINITY ? 0.f : expf((lp - d.mp) * inv) * d.sp;
-    if (d.q && lq != -INFINITY) w = __fsub_rn(w, __fmul_rn(expf((lq - d.mq) * inv), d.sq));
+    float w = power(lp, d.mp, inv) * d.sp;
+    if (d.q) w = __fsub_rn(w, __fmul_rn(power(lq, d.mq, inv), d.sq));
     return v == d.without || !(w > 0.f) ? 0.f : w;
 }
-// the weights of a block of numbers from b on, ahead of `end`: a thread's sums of four each, numbers b + 1024 p + 4 tid .. + 3
-__device__ __forceinline__ void block_weights(const drawn_row &d, float inv, int64_t b, int64_t end, bool vec_t, bool vec_d, double (&sum)[kPasses]) {
-    float4 lp[kPasses], lq[kPasses];
-#pragma unroll
-    for (int p = 0; p < kPasses; p++) {
-        const int64_t v = b + 4 * kThreads * p + 4 * threadIdx.x;
-        lp[p] = lq[p] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (b + 4 * kThreads * p < end) {
-            lp[p] = load4(d.p, v, end, vec_t);
-            if (d.q) lq[p] = load4(d.q, v, end, vec_d);
-        }
-    }
-#pragma unroll
-    for (int p = 0; p < kPasses; p++) {
-        const int64_t v = b + 4 * kThreads * p + 4 * threadIdx.x;
-        sum[p] = 0.0;
-        if (b + 4 * kThreads * p < end)
-            sum[p] = (double)((weight(d, inv, lp[p].x, lq[p].x, v) + weight(d, inv, lp[p].y, lq[p].y, v + 1)) +
-                              (weight(d, inv, lp[p].z, lq[p].z, v + 2) + weight(d, inv, lp[p].w, lq[p].w, v + 3)));
-    }
+__device__ __forceinline__ float weights(const drawn_row &d, float inv, float4 lp, float4 lq, int64_t v) { // of four numbers
+    return (weight(d, inv, lp.x, lq.x, v) + weight(d, inv, lp.y, lq.y, v + 1)) + (weight(d, inv, lp.z, lq.z, v + 2) + weight(d, inv, lp.w, lq.w, v + 3));
 }
+__device__ __forceinline__ float pick4(float4 x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; }
 
 struct place {
     int at;               // the first of the sums at which their running sum exceeds `to`; should none (rounding), the last with anything in it, or -1
@@ -246,10 +236,9 @@ template <int E> __device__ __forceinline__ place place_of(const double (&sum)[E
 }
 
 template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_pick_kernel(const __grid_constant__ verify_args a) {
-    constexpr int kWarps = kThreads / 32;
     __shared__ int s_first, s_extra;
     __shared__ bool s_last;
-    __shared__ double s_sum[2][kPasses * kWarps];
+    __shared__ double s_sum[2][kWarps];
     __shared__ row_stats s_p, s_q;
     step_wait();
     const int seq = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -306,69 +295,84 @@ template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_pick_k
                 d.without = a.drafted[r];
             }
         }
-        const int64_t v0 = blockIdx.x * a.piece, v1 = min(a.V, v0 + a.piece);
-        double sum = 0.0, part[kPasses];
+        const int64_t share = a.piece / kWarps; // a warp's part of a piece: a multiple of 4
+        const int64_t v0 = blockIdx.x * a.piece + warp * share, v1 = min(a.V, v0 + share);
+        double *sums = a.sums + (int64_t)seq * a.pieces * kWarps;
+        double sum = 0.0;
         if (valid)
-            for (int64_t b = v0; b < v1; b += kBlock) {
-                block_weights(d, a.inv, b, v1, a.vec_t, a.vec_d, part);
+            for (int64_t b = v0; b < v1; b += 4 * 32 * kPasses) {
+                float4 lp[kPasses], lq[kPasses];
+                const int n = (int)min((int64_t)(4 * 32 * kPasses), v1 - b);
 #pragma unroll
-                for (int p = 0; p < kPasses; p++) sum += part[p];
+                for (int p = 0; p < kPasses; p++) {
+                    lp[p] = lq[p] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (4 * 32 * p < n) {
+                        lp[p] = load4(d.p + b, 4 * 32 * p + 4 * lane, n, a.vec_t);
+                        if (d.q) lq[p] = load4(d.q + b, 4 * 32 * p + 4 * lane, n, a.vec_d);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < kPasses; p++)
+                    if (4 * 32 * p < n) sum += (double)weights(d, a.inv, lp[p], lq[p], b + 4 * 32 * p + 4 * lane);
             }
         sum = warp_sum_f64(sum);
-        if (lane == 0) s_sum[0][warp] = sum;
+        if (lane == 0) {
+            sums[blockIdx.x * kWarps + warp] = sum;
+            __threadfence();
+        }
         __syncthreads();
         if (tid == 0) {
-            for (int w = 1; w < kWarps; w++) sum += s_sum[0][w];
-            a.sums[(int64_t)seq * a.pieces + blockIdx.x] = sum;
-            __threadfence();
             s_last = atomicAdd(&a.done[seq], 1u) == gridDim.x - 1;
             s_extra = -1;
         }
         __syncthreads();
         if (!s_last) return;
         __threadfence();
-        // ---- the last one: the piece whose running sum exceeds u times the whole, then the place in it; every warp finds the same piece
+        // ---- the last one: the piece whose running sum exceeds u times the whole, then the warp's part of it; every warp finds the same
         double piece_sum[kMaxPieces / 32];
 #pragma unroll
         for (int e = 0; e < kMaxPieces / 32; e++) {
             const int c = kMaxPieces / 32 * lane + e;
-            piece_sum[e] = c < a.pieces ? __ldcg(a.sums + (int64_t)seq * a.pieces + c) : 0.0;
+            piece_sum[e] = 0.0;
+            if (c < a.pieces) {
+                double x[kWarps];
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) x[w] = __ldcg(sums + c * kWarps + w);
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) piece_sum[e] += x[w];
+            }
         }
         const double u = (double)a.u[r0 + drafts];
         int64_t b0 = 0, b1 = 0;
-        double run = 0.0, to = u * place_of(piece_sum, 0.0, 0.0).whole;
-        const place in = place_of(piece_sum, 0.0, to);
-        if (valid && in.at >= 0) {
-            b0 = in.at * a.piece, b1 = min(a.V, b0 + a.piece), run = in.before;
+        double run = 0.0, to = u * place_of(piece_sum, 0.0, INFINITY).whole;
+        const place piece = place_of(piece_sum, 0.0, to);
+        if (valid && piece.at >= 0) {
+            const double part[1] = {lane < kWarps ? __ldcg(sums + piece.at * kWarps + lane) : 0.0};
+            const place in = place_of(part, piece.before, to);
+            b0 = piece.at * a.piece + in.at * share, b1 = min(a.V, b0 + share), run = in.before;
         } else if (valid && (d.q || d.without >= 0)) { // rounding left nothing of p - q: from p, one sum over the whole row
             d.q = nullptr, d.without = -1, d.sp = 1.f;
             b1 = a.V, to = u * t.s;
         }
-        // a block at a time: the sums of its passes and warps in order, then the lanes' in the one where the running sum exceeds and the four numbers of that lane
+        // four numbers a thread at a time: the warps' sums in order, then the lanes' in the one where the running sum exceeds and the four numbers of that lane
         int turn = 0;
-        for (int64_t b = b0; b < b1; b += kBlock, turn ^= 1) {
-            block_weights(d, a.inv, b, b1, a.vec_t, a.vec_d, part);
-#pragma unroll
-            for (int p = 0; p < kPasses; p++) {
-                const double w = warp_sum_f64(part[p]);
-                if (lane == 0) s_sum[turn][p * kWarps + warp] = w;
-            }
+        for (int64_t b = b0; b < b1; b += 4 * kThreads, turn ^= 1) {
+            const int64_t v = b + 4 * tid;
+            const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const int n = (int)min((int64_t)(4 * kThreads), b1 - b);
+            const float4 lp = load4(d.p + b, 4 * tid, n, a.vec_t), lq = d.q ? load4(d.q + b, 4 * tid, n, a.vec_d) : none;
+            const double mine[1] = {(double)weights(d, a.inv, lp, lq, v)}, all = warp_sum_f64(mine[0]);
+            if (lane == 0) s_sum[turn][warp] = all;
             __syncthreads();
-            const double two[2] = {s_sum[turn][2 * lane], s_sum[turn][2 * lane + 1]};
-            const place block = place_of(two, run, to);
-            if (block.at >= 0 && block.at % kWarps == warp) {
-                double mine[1] = {0.0};
-#pragma unroll
-                for (int p = 0; p < kPasses; p++)
-                    if (p == block.at / kWarps) mine[0] = part[p];
+            const double part[1] = {lane < kWarps ? s_sum[turn][lane] : 0.0};
+            const place block = place_of(part, run, to);
+            if (block.at == warp) {
                 const place four = place_of(mine, block.before, to);
                 if (lane == four.at) {
                     double upto = four.before;
-                    const int64_t v = b + 4 * kThreads * (block.at / kWarps) + 4 * tid;
-                    const float4 lp = load4(d.p, v, b1, a.vec_t), lq = d.q ? load4(d.q, v, b1, a.vec_d) : lp;
-                    const float x[4] = {lp.x, lp.y, lp.z, lp.w}, y[4] = {lq.x, lq.y, lq.z, lq.w};
+#pragma unroll 1
                     for (int e = 0; e < 4; e++) {
-                        const float w = weight(d, a.inv, x[e], y[e], v + e);
+                        const float w = weight(d, a.inv, pick4(lp, e), pick4(lq, e), v + e);
                         if (!(w > 0.f)) continue;
                         s_extra = (int)(v + e); // the last one with a weight, so far
                         upto += (double)w;
@@ -391,7 +395,7 @@ template <bool GREEDY> __global__ void __launch_bounds__(kThreads) verify_pick_k
 extern "C" {
 
 size_t ggb_draft_verify_scratch_bytes(int64_t R, int n_seq) {
-    return (size_t)R * 2 * kMaxPieces * sizeof(piece_stats) + (size_t)n_seq * (kMaxPieces * sizeof(double) + sizeof(unsigned));
+    return (size_t)R * 2 * kMaxPieces * sizeof(piece_stats) + (size_t)n_seq * (kMaxPieces * kWarps * sizeof(double) + sizeof(unsigned));
 }
 
 int ggb_op_draft_verify(const float *target, int64_t ld_target, const float *draft, int64_t ld_draft, int64_t V, int64_t R, int n_seq, const int32_t *starts,
@@ -401,7 +405,7 @@ int ggb_op_draft_verify(const float *target, int64_t ld_target, const float *dra
     GGB_CHECK_ARG(V > 0 && V < (1ll << 31) - (1 << 20) && R > 0 && R <= 65535 && n_seq > 0 && n_seq <= 65535, "draft_verify: %lld rows of %lld numbers, %d sequences", (long long)R,
                   (long long)V, n_seq);
     GGB_CHECK_ARG(ld_target >= V && (!draft || ld_draft >= V), "draft_verify: rows of %lld numbers overlap", (long long)V);
-    GGB_CHECK_ARG(temperature >= 0.f && temperature <= 3.0e38f && (temperature == 0.f || 1.0f / temperature <= 3.0e38f), "draft_verify: a temperature of %g", (double)temperature);
+    GGB_CHECK_ARG(temperature >= 0.f && temperature <= 3.0e38f && (temperature == 0.f || 1.5f / temperature <= 3.0e38f), "draft_verify: a temperature of %g", (double)temperature);
     GGB_CHECK_ARG((uintptr_t)scratch % 16 == 0 && scratch_bytes >= ggb_draft_verify_scratch_bytes(R, n_seq), "draft_verify: %zu bytes of scratch, %zu needed on a 16-byte boundary",
                   scratch_bytes, ggb_draft_verify_scratch_bytes(R, n_seq));
     const bool greedy = temperature == 0.f;
@@ -410,14 +414,14 @@ int ggb_op_draft_verify(const float *target, int64_t ld_target, const float *dra
     const int64_t sides = dr ? 2 : 1;
     int64_t piece = 8192;
     while (piece > 2048 && R * sides * ((V + piece - 1) / piece) < 2 * ggb_sm_count()) piece /= 2;
-    piece = std::max(piece, ((V + kMaxPieces - 1) / kMaxPieces + 3) / 4 * 4);
+    piece = std::max(piece, ((V + kMaxPieces - 1) / kMaxPieces + 4 * kWarps - 1) / (4 * kWarps) * (4 * kWarps));
     verify_args a{};
     a.target = target, a.draft = dr, a.ld_t = ld_target, a.ld_d = ld_draft, a.V = V, a.R = R, a.piece = piece, a.n_seq = n_seq, a.pieces = (int)((V + piece - 1) / piece);
-    a.starts = starts, a.drafted = drafted, a.u = u, a.inv = greedy ? 0.f : 1.0f / temperature, a.inv64 = greedy ? 0.0 : 1.0 / (double)temperature, a.tokens = tokens,
+    a.starts = starts, a.drafted = drafted, a.u = u, a.inv = greedy ? 0.f : (float)(1.4426950408889634 / (double)temperature), a.inv64 = greedy ? 0.0 : 1.0 / (double)temperature, a.tokens = tokens,
     a.accepted = n_accepted;
     a.stats = (piece_stats *)scratch;
     a.sums = (double *)(a.stats + R * 2 * kMaxPieces);
-    a.done = (unsigned *)(a.sums + (int64_t)n_seq * kMaxPieces);
+    a.done = (unsigned *)(a.sums + (int64_t)n_seq * kMaxPieces * kWarps);
     a.vec_t = (uintptr_t)target % 16 == 0 && ld_target % 4 == 0, a.vec_d = (uintptr_t)dr % 16 == 0 && ld_draft % 4 == 0;
     const dim3 grid((unsigned)a.pieces, (unsigned)R, (unsigned)sides), pick(greedy ? 1u : (unsigned)a.pieces, (unsigned)n_seq);
     if (greedy) {
