@@ -80,27 +80,65 @@ template <int N> __device__ __forceinline__ void turned_piece(const float *x, in
 
 __device__ __forceinline__ bool piece_fits(int vec, int n, int d, int rot, int halves) { return vec && (d >= rot || (rot % n == 0 && (!halves || (rot / 2) % n == 0))); }
 
-template <int CODE> __global__ void __launch_bounds__(512) kv8_store_kernel(const __grid_constant__ store_args a) {
+template <int CODE> __global__ void __launch_bounds__(512, 2) kv8_store_kernel(const __grid_constant__ store_args a) {
     __shared__ unsigned s_max[2];
     using code = kv8_code<CODE>;
     step_wait();
     const int tid = threadIdx.x;
     if (blockIdx.x >= a.kv_ctas) { // ---- the queries of a token
+        // A thread has the same four numbers of every n-th head, so that it loads their cosines and sines once; the heads' numbers are asked for four at a time, the
+        // first ones before the token's sequence is looked for
         const int64_t t = blockIdx.x - a.kv_ctas;
+        const int quads = a.D / 4, n = blockDim.x / quads, h0 = tid / quads, d = 4 * (tid - h0 * quads);
+        const float *row = a.q + t * a.ld + d;
+        float *out = a.q_out + t * a.H * a.D + d;
+        const int half = a.rot / 2;
+        const bool turns = d < a.rot, piece = piece_fits(a.vec, 4, d, a.rot, a.halves), first = a.halves ? d < half : true;
+        const int other = turns && a.halves ? (first ? half : -half) : 0;
+        constexpr int U = 4;
+        float4 x[U], o[U];
+        auto ask = [&](int h) {
+            if (!piece || h0 >= n) return;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (h + u * n < a.H) {
+                    x[u] = *reinterpret_cast<const float4 *>(row + (h + u * n) * a.D);
+                    if (other) o[u] = *reinterpret_cast<const float4 *>(row + (h + u * n) * a.D + other);
+                }
+        };
+        ask(h0);
         if (t >= a.starts[a.n_seq]) return;
         const int s = last_not_behind(a.n_seq, t, [&](int i) { return (int64_t)a.starts[i]; });
         const int64_t pos = (int64_t)a.pos0[s] + (t - a.starts[s]);
-        const float *cs = a.cs + pos * a.rot, *row = a.q + t * a.ld;
-        float *out = a.q_out + t * a.H * a.D;
-        for (int e = 4 * tid; e < a.H * a.D; e += 4 * blockDim.x) {
-            const int h = e / a.D, d = e - h * a.D; // D is a multiple of 16
-            float y[4];
-            if (piece_fits(a.vec, 4, d, a.rot, a.halves)) {
-                turned_piece<4>(row + h * a.D, d, a.rot, a.halves, cs, y);
-                *reinterpret_cast<float4 *>(out + e) = make_float4(y[0] * a.scale, y[1] * a.scale, y[2] * a.scale, y[3] * a.scale);
-            } else {
+        const float *cs = a.cs + pos * a.rot;
+        if (h0 >= n) return;
+        if (!piece) { // odd strides, or a turn that ends inside
+            for (int h = h0; h < a.H; h += n)
 #pragma unroll
-                for (int u = 0; u < 4; u++) out[e + u] = turned(row + h * a.D, d + u, a.rot, a.halves, cs) * a.scale;
+                for (int u = 0; u < 4; u++) out[h * a.D + u] = turned(row - d + h * a.D, d + u, a.rot, a.halves, cs) * a.scale;
+            return;
+        }
+        float4 c0, c1;
+        if (turns) {
+            const float4 *c4 = reinterpret_cast<const float4 *>(cs + (a.halves ? 2 * (first ? d : d - half) : d));
+            c0 = c4[0];
+            if (a.halves) c1 = c4[1];
+        }
+        for (int h = h0; h < a.H; h += U * n) {
+            if (h != h0) ask(h);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float4 y = x[u];
+                if (turns) {
+                    if (!a.halves) {
+                        y = make_float4(x[u].x * c0.x - x[u].y * c0.y, x[u].y * c0.x + x[u].x * c0.y, x[u].z * c0.z - x[u].w * c0.w, x[u].w * c0.z + x[u].z * c0.w);
+                    } else if (first) {
+                        y = make_float4(x[u].x * c0.x - o[u].x * c0.y, x[u].y * c0.z - o[u].y * c0.w, x[u].z * c1.x - o[u].z * c1.y, x[u].w * c1.z - o[u].w * c1.w);
+                    } else {
+                        y = make_float4(x[u].x * c0.x + o[u].x * c0.y, x[u].y * c0.z + o[u].y * c0.w, x[u].z * c1.x + o[u].z * c1.y, x[u].w * c1.z + o[u].w * c1.w);
+                    }
+                }
+                if (h + u * n < a.H) *reinterpret_cast<float4 *>(out + (h + u * n) * a.D) = make_float4(y.x * a.scale, y.y * a.scale, y.z * a.scale, y.w * a.scale);
             }
         }
         return;
