@@ -71,6 +71,7 @@ struct attn_args {
     float *part;    // [CTA][2][rows][Dv + 2], or null: an item a CTA
     int4 *desc;     // [CTA][2], of an item that begins or goes on here and ends elsewhere: sequence (or -1), rows, key head, first row; first and last CTA that have it, first token
     int vec_q, vec_out, vec_gate; // queries, results, rows of the gate begin on a 16-byte boundary
+    int64_t positions; // that a page table has room for
     int *wait_error;
 };
 // four codes as two pairs of fp16 numbers.  int8: code + 128 behind the bits of 1024, less 1152

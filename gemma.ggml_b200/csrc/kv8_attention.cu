@@ -673,7 +673,7 @@ template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
     const int64_t groups = (max_new * (a.H / a.G) + Z::R - 1) / Z::R;
     GGB_CHECK_ARG(max_new * (a.H / a.G) < (1ll << 30) && a.n_seq * groups * a.G < (1ll << 31), "kv8_attn: too many sequences, tokens and heads for a launch");
-    GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.table_ld * a.B + a.keep) / Z::tile + 4) < (1ll << 31), "kv8_attn: too many positions for a launch"); // the units of a deal, at most
+    GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.positions + a.keep) / Z::tile + 4) < (1ll << 31), "kv8_attn: too many positions for a launch"); // the units of a deal, at most
     a.groups = (int)groups;
     auto k = kv8_step_kernel<CODE, P, NT, PARTS>;
     int rc = ggb_allow_smem(k, Z::smem);
@@ -745,10 +745,11 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
     GGB_CHECK_ARG((uintptr_t)cache % 16 == 0, "kv8_attn: the cache must begin on a 16-byte boundary");
     GGB_CHECK_ARG(!scratch || ((uintptr_t)scratch % 16 == 0 && scratch_bytes >= part_bytes(Dv)), "kv8_attn: %zu bytes of scratch, %zu needed on a 16-byte boundary",
                   scratch_bytes, part_bytes(Dv));
+    const int64_t positions = std::min<int64_t>(table_ld, (1ll << 31) / block_size) * block_size; // (they are 32-bit numbers)
     float *part = (float *)scratch;
-    const attn_args a{q, (const uint8_t *)cache, tables, table_ld, block_size, n_seq, starts, pos0, H, G, D, Dv, window, window > 0 ? keep_first : 0, softcap, sink, gate, ldg,
+    const attn_args a{q, (const uint8_t *)cache, tables, table_ld, block_size, n_seq, starts, pos0, H, G, D, Dv, window, window > 0 ? std::min<int64_t>(keep_first, positions) : 0, softcap, sink, gate, ldg,
                       kv8_record(D, Dv, block_size), out, 0, 0, 0, part, part ? (int4 *)(part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2)) : nullptr, (uintptr_t)q % 16 == 0,
-                      (uintptr_t)out % 16 == 0, (uintptr_t)gate % 16 == 0 && ldg % 4 == 0, ggb_wait_error_flag()};
+                      (uintptr_t)out % 16 == 0, (uintptr_t)gate % 16 == 0 && ldg % 4 == 0, positions, ggb_wait_error_flag()};
     if (dt == GGB_TYPE_BF16) return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 1>(a, T, max_new) : attend<GGB_KV8_E4M3, 1>(a, T, max_new);
     return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 2>(a, T, max_new) : attend<GGB_KV8_E4M3, 2>(a, T, max_new);
 }

@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
 template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t max_new, unsigned *joins) {
     const int hpg = a.H / a.G;
     const int64_t groups = (max_new * hpg + kTileRows - 1) / kTileRows, items = (T * hpg + kTileRows - 1) / kTileRows * a.G;
-    GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.table_ld * a.B + a.keep) / kTileKeys + kTileBegin + 2) < (1ll << 31), "kv8_attn: too many sequences, tokens, heads and positions for a launch");
+    GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.positions + a.keep) / kTileKeys + kTileBegin + 2) < (1ll << 31), "kv8_attn: too many sequences, tokens, heads and positions for a launch");
     a.groups = (int)groups;
     if (items >= 8 * ggb_sm_count()) a.part = nullptr;
     const size_t smem = std::max((size_t)tile_sizes(PARTS, a.D, a.Dv).smem, kOneCtaSmem);

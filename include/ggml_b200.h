@@ -501,7 +501,7 @@ int ggb_op_diff_attn(int dt, const float *q, const void *cache, const int32_t *b
  *
  * A batch: sequence s < n_seq brings the tokens starts[s] .. starts[s + 1] - 1 (starts[0] = 0; none at all where the two are equal), which take the
  * positions pos0[s], pos0[s] + 1, ...; position j lies in page tables[s * table_ld + j / block_size].  starts, pos0 and tables are device int32 (a captured call
- * replays elsewhere); T is the rows that the buffers hold, and rows behind starts[n_seq] are neither read nor written.  The sequences of a call write to
+ * replays elsewhere); T is the rows that the buffers hold; rows behind starts[n_seq] count for nothing and are left as they are.  The sequences of a call write to
  * pages of their own; a table's entries outside of what a sequence sees and brings are not read. */
 #define GGB_KV8_INT8 1 /* codes -127 .. 127 */
 #define GGB_KV8_E4M3 2 /* 8-bit floating point, up to 448 */
