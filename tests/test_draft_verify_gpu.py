@@ -1,7 +1,7 @@
 """Checked drafts on the GPU against tests/kv8_plain.py.  Decisions are whole numbers: they are the plain form's wherever its nearest decision is further off than what
 fp32 exponentials can move, and otherwise (the borders of a running sum over a whole vocabulary lie closer than that) within what they can move.  An exponential of (l - m)
-/ t is off by 2 steps of 2^-24 of expf and |l - m| / t half steps of its argument; sums of many are nearer than one.  With |l - m| / t below 60 where a weight matters that
-is under 64 * 2^-24 = 4e-6 of itself."""
+/ t is off by 4 steps of 2^-24 (the unit's 2^-22) and by (l - m) / t times the three roundings of its argument (difference, constant, product), 2^-24 each; sums of many are
+nearer than one.  Weights below e^-20 of the largest move nothing here (256,000 of them are 5e-4 of it, off by 1e-5), so that is under 64 * 2^-24 = 4e-6 of itself."""
 import ctypes as C
 
 import numpy as np
@@ -172,3 +172,22 @@ def test_what_is_refused(gpu):
                 dict(nbytes=need - 1), dict(scratch=p + 8)):
         assert lib.ggb_op_draft_verify(*{**ok, **bad}.values()) == -2, bad
         assert b"draft_verify" in lib.ggb_last_error()
+
+
+@pytest.mark.parametrize("V", [524288 + 32, 600001])
+@pytest.mark.parametrize("t", [1.0, 0.0])
+def test_vocabularies_of_more_than_64_pieces(gpu, V, t):
+    r = np.random.default_rng(30)
+    target, draft, starts, u = inputs(r, [3, 1], V)
+    drafted = i32(target.argmax(1))
+    want, acc, near = P.verify(target, draft, starts, drafted, u, t)
+    got, accepted = run(gpu, target, draft, starts, drafted, u, t, ld=V + 3)
+    assert np.array_equal(got, want) and np.array_equal(accepted, acc) if near > NEAR else P.agrees(got, accepted, target, draft, starts, drafted, u, t, NEAR)
+
+
+def test_a_long_row_where_nothing_is_left_of_the_difference(gpu):
+    """p = q over 40,000 tokens, u = 1: drawn from p, whose even weights add up exactly"""
+    V = 40000
+    target = np.zeros((4, V), np.float32)
+    got, acc = run(gpu, target, target, [0, 2, 4], [5, 0, 5, 0], np.array([1.0, 0.9, 1.0, 0.125], np.float32), 1.0)
+    assert list(acc) == [0, 0] and list(got) == [int(np.floor(np.float64(np.float32(0.9)) * V)), -1, V // 8, -1]
