@@ -512,9 +512,17 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                             halves_of<CODE>(__byte_perm(vx[0][w], vx[1][w], sel), a0, a1);
                             halves_of<CODE>(__byte_perm(vx[2][w], vx[3][w], sel), a2, a3);
 #pragma unroll
-                            for (int part = PARTS - 1; part >= 0; part--)
+                            for (int t = 0; t < NT; t++) {
+                                if (PARTS == 1) {
+                                    mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[u][0][t][0], pb[u][0][t][1]);
+                                } else { // tensor cores cut their sums short, always towards zero: not the long one, which is rounded to the nearest
+                                    float z4[4];
+                                    mma16816_first(z4, a0, a1, a2, a3, pb[u][PARTS - 1][t][0], pb[u][PARTS - 1][t][1]);
+                                    mma16816(z4, a0, a1, a2, a3, pb[u][0][t][0], pb[u][0][t][1]);
 #pragma unroll
-                                for (int t = 0; t < NT; t++) mma16816(o[c * 8 + 2 * w + y][t], a0, a1, a2, a3, pb[u][part][t][0], pb[u][part][t][1]);
+                                    for (int e = 0; e < 4; e++) o[c * 8 + 2 * w + y][t][e] += z4[e];
+                                }
+                            }
                         }
                 }
             used += Z::U;

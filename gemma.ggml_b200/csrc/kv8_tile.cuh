@@ -27,6 +27,8 @@ constexpr int kSoftWarps = 8, kCodeWarps = 8, kTileThreads = 32 * (kSoftWarps + 
 // registers: five groups of four warps are launched with 96 a thread, of which the weights' take 152 and the others 64 and 48 (2 x 152 + 2 x 64 + 48 = 5 x 96)
 constexpr int kSoftRegs = 152, kCodeRegs = 64, kMmaRegs = 48;
 constexpr int kAhead = 3; // tiles of codes asked for
+// tensor cores cut their sums short, always towards zero: with fp32 results what a chain of so many tiles has summed up is added, rounded to the nearest, to the rest in memory
+constexpr int kChain = 16;
 enum { T_K_FULL = 0, T_K_FREE = 16, T_V_FULL = 32, T_V_FREE = 48, T_S_FULL = 64, T_P_FULL = 80, T_DONE = 96, T_Q_FULL = 104, T_S_FREE = 112, T_SLOT = 128, T_DEAD = 132, T_RAW = 136, T_RAW_FREE = 168 };
 // tensor memory: two groups' scores, their weights, their output
 constexpr uint32_t kScoreCol = 0, kWeightCol = 128, kOutCol = 256;
@@ -104,7 +106,7 @@ template <int PARTS, int KS> __device__ __forceinline__ void tile_products(const
         tc_fence_after();
         const uint32_t o = m.tmem + kOutCol + s * m.Dv, p = m.tmem + kWeightCol + s * 64, vl = v_lo + ((s * m.v_stage) >> 4);
 #pragma unroll
-        for (int part = PARTS - 1; part >= 0; part--) umma_ts_k4(o, p + part * 32, vl, 128, id_o, part < PARTS - 1 ? 1u : t >= 2);
+        for (int part = PARTS - 1; part >= 0; part--) umma_ts_k4(o, p + part * 32, vl, 128, id_o, part < PARTS - 1 ? 1u : (PARTS == 1 ? t : t % kChain) >= 2);
         umma_arrive(m.bars + T_V_FREE + 8 * s);
     }
     umma_arrive(m.bars + T_DONE);
@@ -413,161 +415,194 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
             const float rowf = srow[r], cap = a.cap * kLog2e, inv_cap = a.cap > 0.f ? kLn2 / a.cap : 0.f;
             float m = kNone, l = 0.f, vref = 0.f, vinv = 0.f;
             bool lost = false;
-            for (int k = grp; k < n; k += 2) {
-                const int t = tile + k, j0 = first_of(t);
-                const bool kept = t < it.kt, whole = kept ? j0 + kTileKeys <= it.n_keep : j0 >= whole_from && j0 + kTileKeys - 1 <= it.i0;
-                if (!wait_long(bars + T_S_FULL + 8 * grp, (ph + (k >> 1)) & 1, dead)) lost = true;
-                tc_fence_after();
-                const float4 *sc4 = reinterpret_cast<const float4 *>(scales + ((ph0 + ph1 + k) & 15) * 4);
-                const float4 sa = sc4[0], sb = sc4[1];
-                const float ks[4] = {sa.x, sa.z, sb.x, sb.z}, vs[4] = {sa.y, sa.w, sb.y, sb.w};
-                float y[4][16], f[4], mx = kNone;
-                tmem_load32(ts, reinterpret_cast<uint32_t *>(y[0]));
-                tmem_load32(ts + 32, reinterpret_cast<uint32_t *>(y[2]));
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bars + T_S_FREE + 8 * grp);
-                // a score is its product times f; where something is in between, it is taken into the scores and f is one
-#pragma unroll
-                for (int g = 0; g < 4; g++) f[g] = rowf * ks[g];
-                if (a.cap > 0.f || !whole) {
-#pragma unroll
-                    for (int g = 0; g < 4; g++) {
-#pragma unroll
-                        for (int c = 0; c < 16; c++) y[g][c] *= f[g];
-                        f[g] = 1.f;
-                        if (a.cap > 0.f) tile_attn::soft_cap16(y[g], cap, inv_cap);
-                    }
-                    if (!whole) { // positions [from, upto) of the tile, and of those below `from` the kept ones
-                        const int upto = i < 0 ? 0 : (kept ? it.n_keep : i + 1) - j0, from = (kept ? 0 : lo) - j0, keep = kept ? 0 : (int)min(a.keep, (int64_t)lo) - j0, low = kept ? 0 : it.lo - j0;
-#pragma unroll
-                        for (int g = 0; g < 4; g++)
-#pragma unroll
-                            for (int c = 0; c < 16; c++) {
-                                const int j = 16 * g + c;
-                                if (!(j < upto && j >= low && (j >= from || j < keep))) y[g][c] = -INFINITY;
-                            }
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    float big[2] = {y[g][0], y[g][1]};
-#pragma unroll
-                    for (int c = 2; c < 16; c++) big[c & 1] = fmaxf(big[c & 1], y[g][c]);
-                    mx = fmaxf(mx, fmaxf(big[0], big[1]) * f[g]);
-                }
-                float over = 1.f;
-                if (mx > m + 8.f) {
-                    over = exp2f(m - mx);
-                    m = mx, l *= over;
-                }
-                const float most_v = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-                if (most_v > 64.f * vref) {
-                    over *= vref / most_v;
-                    vref = most_v, vinv = 1.f / most_v;
-                }
-                // (from here on the weights that this tile's go over have been read, and the output that they went into is there: tile k - 2's products)
-                if (k >= 2 && !wait_long(bars + T_V_FREE + 8 * grp, (ph + (k >> 1) - 1) & 1, dead)) lost = true;
-                tc_fence_after();
-                if (k >= 2 && __any_sync(0xffffffffu, over != 1.f)) {
-#pragma unroll 1
-                    for (int c = 0; c < a.Dv; c += 16) {
-                        uint32_t o[16];
-                        tmem_load16(to + c, o);
-#pragma unroll
-                        for (int u = 0; u < 16; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * over);
-                        tmem_store16(to + c, o);
-                    }
-                }
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    f32x2 sum[2] = {0, 0};
-                    const float rel = vs[g] > 0.f ? fmaxf(vs[g] * vinv, 0x1p-40f) : 1.f; // (a scale of zero: values of zero.  2^-40 of another value's scale: nothing)
-                    // one part: the scale goes with the exponent, and out of the sum again
-                    const float power = PARTS == 1 ? lg2_approx(rel) : 0.f, shift = power - m;
-                    uint32_t hi[8], lo2[8];
-#pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        const float2 t2 = unpack2(fma2(pack2(y[g][2 * c], y[g][2 * c + 1]), pack2(f[g], f[g]), pack2(shift, shift)));
-                        f32x2 w = pack2(ex2_approx(t2.x), ex2_approx(t2.y));
-                        sum[c & 1] = add2(sum[c & 1], w);
-                        if (PARTS == 2) w = mul2(w, pack2(rel, rel));
-                        const float2 wv = unpack2(w);
-                        hi[c] = half2_bits(wv.x, wv.y);
-                        if (PARTS == 2) {
-                            const float2 back = half2_floats(hi[c]);
-                            lo2[c] = half2_bits(wv.x - back.x, wv.y - back.y);
-                        }
-                    }
-                    tmem_store8(tw + 8 * g, hi);
-                    if (PARTS == 2) tmem_store8(tw + 32 + 8 * g, lo2);
-                    const float2 s2 = unpack2(add2(sum[0], sum[1]));
-                    l = PARTS == 1 ? fmaf(s2.x + s2.y, ex2_approx(-power), l) : l + (s2.x + s2.y);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bars + T_P_FULL + 8 * grp);
-                if (lost) break;
-            }
-            // ---- both groups' sums meet
-            wait_long(bars + T_DONE, pieces & 1, dead);
-            tc_fence_after();
-            bar_sync(3, 32 * kSoftWarps); // the tables are no longer read
-            st[3 * grp * kTileRows + r] = l, st[(3 * grp + 1) * kTileRows + r] = m, st[(3 * grp + 2) * kTileRows + r] = vref;
-            bar_sync(3, 32 * kSoftWarps);
-            const float m0 = st[kTileRows + r], m1 = st[4 * kTileRows + r], M = fmaxf(m0, m1), g0 = exp2f(m0 - M), g1 = n > 1 ? exp2f(m1 - M) : 0.f;
-            const float L = fmaf(st[r], g0, n > 1 ? st[3 * kTileRows + r] * g1 : 0.f);
-            const float f0 = g0 * st[2 * kTileRows + r], f1 = g1 * st[5 * kTileRows + r];
             const bool whole_item = n == it.n;
             const int row = it.row0 + r, tq = row / hpg, h = x.head * hpg + (row - tq * hpg);
-            const int64_t t = it.t0 + tq;
+            const int64_t t_row = it.t0 + tq;
             float *part = whole_item ? nullptr : a.part + (((int64_t)blockIdx.x * 2 + (tile == 0)) * kTileRows + r) * (a.Dv + 2);
-            const row_end end(a, r < it.rows ? h : 0, M, L);
+            float M = kNone, L = 0.f; // of the chains so far
+            int k = grp;
+            for (int upto = PARTS == 1 ? n : min(n, kChain);; upto = min(n, upto + kChain)) {
+                for (; k < upto; k += 2) {
+                    const int t = tile + k, j0 = first_of(t);
+                    const bool kept = t < it.kt, whole = kept ? j0 + kTileKeys <= it.n_keep : j0 >= whole_from && j0 + kTileKeys - 1 <= it.i0;
+                    if (!wait_long(bars + T_S_FULL + 8 * grp, (ph + (k >> 1)) & 1, dead)) lost = true;
+                    tc_fence_after();
+                    const float4 *sc4 = reinterpret_cast<const float4 *>(scales + ((ph0 + ph1 + k) & 15) * 4);
+                    const float4 sa = sc4[0], sb = sc4[1];
+                    const float ks[4] = {sa.x, sa.z, sb.x, sb.z}, vs[4] = {sa.y, sa.w, sb.y, sb.w};
+                    float y[4][16], f[4], mx = kNone;
+                    tmem_load32(ts, reinterpret_cast<uint32_t *>(y[0]));
+                    tmem_load32(ts + 32, reinterpret_cast<uint32_t *>(y[2]));
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars + T_S_FREE + 8 * grp);
+                    // a score is its product times f; where something is in between, it is taken into the scores and f is one
+#pragma unroll
+                    for (int g = 0; g < 4; g++) f[g] = rowf * ks[g];
+                    if (a.cap > 0.f || !whole) {
+#pragma unroll
+                        for (int g = 0; g < 4; g++) {
+#pragma unroll
+                            for (int c = 0; c < 16; c++) y[g][c] *= f[g];
+                            f[g] = 1.f;
+                            if (a.cap > 0.f) tile_attn::soft_cap16(y[g], cap, inv_cap);
+                        }
+                        if (!whole) { // positions [from, upto) of the tile, and of those below `from` the kept ones
+                            const int upto = i < 0 ? 0 : (kept ? it.n_keep : i + 1) - j0, from = (kept ? 0 : lo) - j0, keep = kept ? 0 : (int)min(a.keep, (int64_t)lo) - j0, low = kept ? 0 : it.lo - j0;
+#pragma unroll
+                            for (int g = 0; g < 4; g++)
+#pragma unroll
+                                for (int c = 0; c < 16; c++) {
+                                    const int j = 16 * g + c;
+                                    if (!(j < upto && j >= low && (j >= from || j < keep))) y[g][c] = -INFINITY;
+                                }
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        float big[2] = {y[g][0], y[g][1]};
+#pragma unroll
+                        for (int c = 2; c < 16; c++) big[c & 1] = fmaxf(big[c & 1], y[g][c]);
+                        mx = fmaxf(mx, fmaxf(big[0], big[1]) * f[g]);
+                    }
+                    float over = 1.f;
+                    if (mx > m + 8.f) {
+                        over = exp2f(m - mx);
+                        m = mx, l *= over;
+                    }
+                    const float most_v = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+                    if (most_v > 64.f * vref) {
+                        over *= vref / most_v;
+                        vref = most_v, vinv = 1.f / most_v;
+                    }
+                    // (from here on the weights that this tile's go over have been read, and the output that they went into is there: tile k - 2's products)
+                    if (k >= 2 && !wait_long(bars + T_V_FREE + 8 * grp, (ph + (k >> 1) - 1) & 1, dead)) lost = true;
+                    tc_fence_after();
+                    if ((PARTS == 1 ? k : k % kChain) >= 2 && __any_sync(0xffffffffu, over != 1.f)) {
 #pragma unroll 1
-            for (int cb = grp; cb < a.Dv / 16; cb += 2) {
-                const int64_t at = (int64_t)h * a.Dv + 16 * cb;
-                float4 gt[4];
-                const float *gate = a.gate + t * a.ldg + at;
-                if (whole_item && a.gate && r < it.rows)
+                        for (int c = 0; c < a.Dv; c += 16) {
+                            uint32_t o[16];
+                            tmem_load16(to + c, o);
 #pragma unroll
-                    for (int u = 0; u < 4; u++) gt[u] = a.vec_gate ? *reinterpret_cast<const float4 *>(gate + 4 * u) : make_float4(gate[4 * u], gate[4 * u + 1], gate[4 * u + 2], gate[4 * u + 3]);
-                uint32_t o0[16], o1[16];
-                tmem_load16(tmem + lanes + kOutCol + 16 * cb, o0);
-                if (n > 1) tmem_load16(tmem + lanes + kOutCol + a.Dv + 16 * cb, o1);
-                if (r >= it.rows) continue;
-                float v[16];
+                            for (int u = 0; u < 16; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * over);
+                            tmem_store16(to + c, o);
+                        }
+                    }
 #pragma unroll
-                for (int u = 0; u < 16; u++) {
-                    v[u] = __uint_as_float(o0[u]) * f0;
-                    if (n > 1) v[u] = fmaf(__uint_as_float(o1[u]), f1, v[u]);
+                    for (int g = 0; g < 4; g++) {
+                        f32x2 sum[2] = {0, 0};
+                        const float rel = vs[g] > 0.f ? fmaxf(vs[g] * vinv, 0x1p-40f) : 1.f; // (a scale of zero: values of zero.  2^-40 of another value's scale: nothing)
+                        // one part: the scale goes with the exponent, and out of the sum again
+                        const float power = PARTS == 1 ? lg2_approx(rel) : 0.f, shift = power - m;
+                        uint32_t hi[8], lo2[8];
+#pragma unroll
+                        for (int c = 0; c < 8; c++) {
+                            const float2 t2 = unpack2(fma2(pack2(y[g][2 * c], y[g][2 * c + 1]), pack2(f[g], f[g]), pack2(shift, shift)));
+                            f32x2 w = pack2(ex2_approx(t2.x), ex2_approx(t2.y));
+                            sum[c & 1] = add2(sum[c & 1], w);
+                            if (PARTS == 2) w = mul2(w, pack2(rel, rel));
+                            const float2 wv = unpack2(w);
+                            hi[c] = half2_bits(wv.x, wv.y);
+                            if (PARTS == 2) {
+                                const float2 back = half2_floats(hi[c]);
+                                lo2[c] = half2_bits(wv.x - back.x, wv.y - back.y);
+                            }
+                        }
+                        tmem_store8(tw + 8 * g, hi);
+                        if (PARTS == 2) tmem_store8(tw + 32 + 8 * g, lo2);
+                        const float2 s2 = unpack2(add2(sum[0], sum[1]));
+                        l = PARTS == 1 ? fmaf(s2.x + s2.y, ex2_approx(-power), l) : l + (s2.x + s2.y);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bars + T_P_FULL + 8 * grp);
+                    if (lost) break;
                 }
-                if (!whole_item) {
+                // ---- both groups' sums meet, and those of the chains before: these lie where the result goes
+                const bool last = PARTS == 1 || upto == n, more = PARTS == 2 && upto > kChain;
+                if (last) wait_long(bars + T_DONE, pieces & 1, dead);
+                else wait_long(bars + T_V_FREE + 8 * grp, (ph + ((k - 2) >> 1)) & 1, dead);
+                tc_fence_after();
+                bar_sync(3, 32 * kSoftWarps); // the tables are no longer read
+                st[3 * grp * kTileRows + r] = l, st[(3 * grp + 1) * kTileRows + r] = m, st[(3 * grp + 2) * kTileRows + r] = vref;
+                bar_sync(3, 32 * kSoftWarps);
+                const float before = M, m0 = st[kTileRows + r], m1 = n > 1 ? st[4 * kTileRows + r] : kNone;
+                M = fmaxf(fmaxf(m0, m1), before);
+                const float g0 = exp2f(m0 - M), g1 = n > 1 ? exp2f(m1 - M) : 0.f, gb = more ? exp2f(before - M) : 0.f;
+                L = fmaf(st[r], g0, n > 1 ? st[3 * kTileRows + r] * g1 : 0.f) + (more ? L * gb : 0.f);
+                const float f0 = g0 * st[2 * kTileRows + r], f1 = g1 * st[5 * kTileRows + r];
+                const row_end end(a, r < it.rows ? h : 0, M, L);
+#pragma unroll 1
+                for (int cb = grp; cb < a.Dv / 16; cb += 2) {
+                    const int64_t at = (int64_t)h * a.Dv + 16 * cb;
+                    float4 gt[4];
+                    const float *gate = a.gate + t_row * a.ldg + at;
+                    if (last && whole_item && a.gate && r < it.rows)
 #pragma unroll
-                    for (int u = 0; u < 16; u += 2) *reinterpret_cast<float2 *>(part + 16 * cb + u) = make_float2(v[u], v[u + 1]);
-                    continue;
-                }
+                        for (int u = 0; u < 4; u++) gt[u] = a.vec_gate ? *reinterpret_cast<const float4 *>(gate + 4 * u) : make_float4(gate[4 * u], gate[4 * u + 1], gate[4 * u + 2], gate[4 * u + 3]);
+                    uint32_t o0[16], o1[16];
+                    tmem_load16(tmem + lanes + kOutCol + 16 * cb, o0);
+                    if (n > 1) tmem_load16(tmem + lanes + kOutCol + a.Dv + 16 * cb, o1);
+                    if (r >= it.rows) continue;
+                    E *out = reinterpret_cast<E *>(a.out) + t_row * a.H * a.Dv + at;
+                    float v[16];
 #pragma unroll
-                for (int u = 0; u < 16; u++) v[u] *= end.f;
-                if (a.gate) {
+                    for (int u = 0; u < 16; u++) {
+                        v[u] = __uint_as_float(o0[u]) * f0;
+                        if (n > 1) v[u] = fmaf(__uint_as_float(o1[u]), f1, v[u]);
+                    }
+                    if (more) {
+                        if (!whole_item) {
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const float2 p = unpack2(tile_attn::sigmoid_fast2(pack2(gt[u].x, gt[u].y))), s = unpack2(tile_attn::sigmoid_fast2(pack2(gt[u].z, gt[u].w)));
-                        v[4 * u] *= p.x, v[4 * u + 1] *= p.y, v[4 * u + 2] *= s.x, v[4 * u + 3] *= s.y;
+                            for (int u = 0; u < 16; u += 2) {
+                                const float2 b = *reinterpret_cast<const float2 *>(part + 16 * cb + u);
+                                v[u] = fmaf(b.x, gb, v[u]), v[u + 1] = fmaf(b.y, gb, v[u + 1]);
+                            }
+                        } else if (a.vec_out) {
+#pragma unroll
+                            for (int u = 0; u < 16; u += 4) {
+                                const float4 b = *reinterpret_cast<const float4 *>(out + u);
+                                v[u] = fmaf(b.x, gb, v[u]), v[u + 1] = fmaf(b.y, gb, v[u + 1]), v[u + 2] = fmaf(b.z, gb, v[u + 2]), v[u + 3] = fmaf(b.w, gb, v[u + 3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < 16; u++) v[u] = fmaf(*reinterpret_cast<const float *>(out + u), gb, v[u]);
+                        }
+                    }
+                    if (!whole_item) {
+#pragma unroll
+                        for (int u = 0; u < 16; u += 2) *reinterpret_cast<float2 *>(part + 16 * cb + u) = make_float2(v[u], v[u + 1]);
+                        continue;
+                    }
+                    if (last) {
+#pragma unroll
+                        for (int u = 0; u < 16; u++) v[u] *= end.f;
+                        if (a.gate) {
+#pragma unroll
+                            for (int u = 0; u < 4; u++) {
+                                const float2 p = unpack2(tile_attn::sigmoid_fast2(pack2(gt[u].x, gt[u].y))), s = unpack2(tile_attn::sigmoid_fast2(pack2(gt[u].z, gt[u].w)));
+                                v[4 * u] *= p.x, v[4 * u + 1] *= p.y, v[4 * u + 2] *= s.x, v[4 * u + 3] *= s.y;
+                            }
+                        }
+                    }
+                    if (!a.vec_out) {
+#pragma unroll
+                        for (int u = 0; u < 16; u++) out[u] = from_f32<E>(v[u]);
+                    } else if (PARTS == 1) {
+#pragma unroll
+                        for (int u = 0; u < 16; u += 8)
+                            *reinterpret_cast<uint4 *>(out + u) = make_uint4(pack_bf16x2(v[u], v[u + 1]), pack_bf16x2(v[u + 2], v[u + 3]), pack_bf16x2(v[u + 4], v[u + 5]), pack_bf16x2(v[u + 6], v[u + 7]));
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 16; u += 4) *reinterpret_cast<float4 *>(out + u) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
                     }
                 }
-                E *out = reinterpret_cast<E *>(a.out) + t * a.H * a.Dv + at;
-                if (!a.vec_out) {
-#pragma unroll
-                    for (int u = 0; u < 16; u++) out[u] = from_f32<E>(v[u]);
-                } else if (PARTS == 1) {
-#pragma unroll
-                    for (int u = 0; u < 16; u += 8)
-                        *reinterpret_cast<uint4 *>(out + u) = make_uint4(pack_bf16x2(v[u], v[u + 1]), pack_bf16x2(v[u + 2], v[u + 3]), pack_bf16x2(v[u + 4], v[u + 5]), pack_bf16x2(v[u + 6], v[u + 7]));
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 16; u += 4) *reinterpret_cast<float4 *>(out + u) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
-                }
+                if (last) break;
+                l = 0.f, m = kNone, vref = 0.f;
+                tc_fence_before(); // the next chain begins when the other group has read this one's too
+                bar_sync(3, 32 * kSoftWarps);
+                tc_fence_after();
             }
             if (!whole_item && grp == 0 && r < it.rows) *reinterpret_cast<float2 *>(part + a.Dv) = make_float2(M, L);
             if (!whole_item && tile + n < it.n && tid == 0) {

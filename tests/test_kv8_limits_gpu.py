@@ -118,3 +118,19 @@ def test_two_batches_in_one_graph_over_one_workspace(gpu):
         for s, (want, reach) in zip(sides, wants):
             check_attention(F32, from_dt(F32, s["out"], (s["T"], H, D))[:len(want)], want, reach, D, 256)
     lib.ggb_graph_free(graph)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_fp32_results_over_many_positions(gpu, new):
+    """without a workspace a CTA goes through all positions: sums that the tensor cores cut short (by 2^-25 of themselves on average, towards zero, at every step of 16 keys and
+    both parts) may not be the long ones.  64 such steps in a row are 1.9e-6 at most, scores and weights add 30 u = 1.8e-6 (all one way; in fact less): 12,000 positions
+    in one row would be 1500 / 2 steps"""
+    r = np.random.default_rng(16)
+    starts, tables, pages = batch(r, [new], [12000], 64)
+    cache = P.Cache(P.INT8, 1, 64, 64, 64, pages).filled(r)
+    q = f32(r.standard_normal((new, 4, 64)) * 0.2)
+    want, _ = P.attention(cache, q, starts, [12000], np.maximum(tables, 0))
+    got = run_attention(gpu, F32, cache, q, new, starts, [12000], tables, new, scratch=False)
+    assert np.linalg.norm(got - want) < 3.7e-6 * np.linalg.norm(want)
+    got = run_attention(gpu, F32, cache, q, new, starts, [12000], tables, new)
+    assert np.linalg.norm(got - want) < 3.7e-6 * np.linalg.norm(want)
