@@ -1,23 +1,27 @@
 // kv8_attention.cu — grouped-query soft-max attention of a batch of sequences over the 8-bit paged cache (kv8.cuh).
 //
-// Steps of a token or some drafted ones of every sequence, few rows of queries a key head:
+// Steps of a token or some drafted ones of every sequence, few rows of queries a key head (portions of prompts: kv8_tile.cuh):
 //
-// What has to be read are the codes, a byte a number, and a warp turns each into fp16 (exactly: 8 bits fit) once for all query heads of the key head.  Both products are
-// mma.m16n8k16 with the keys, or the value coordinates, as the 16 rows and eight rows of queries as the columns, so no row of an MMA is empty for the usual four to
-// eight query heads of a key head:
+// What has to be read are the codes, a byte a number, and a warp turns each into what its MMAs take once for all query heads of the key head.  Keys, or value coordinates, are
+// the 16 rows of an MMA and eight rows of queries its columns, so no row is empty for the usual four to eight query heads of a key head:
 //
-//   scores   S^T [16 keys][8 rows] = K Q^T, a lane's piece of a key is 16 consecutive codes straight from the cache: the order of a sum's terms is free, and queries
-//            lie in shared memory in the same one
+//   codes    copied by TMA, a group of 16 positions at a time, a stage or more ahead for every warp on its own
+//   scores   S^T [16 keys][8 rows] = K Q^T.  int8 codes: m16n8k32 on integers, a row of queries as three (bf16 results) or four digits to the base 128 whose products are put
+//            together exactly; e4m3: m16n8k16 on fp16 numbers.  A lane's piece of a key is 16 consecutive codes: the order of a sum's terms is free, and queries lie in
+//            shared memory in the same one
 //   weights  in the registers that the scores are in: 2^(s - m); a kept maximum is followed only when a score exceeds it by 8 (a vote, no shuffles otherwise)
-//   output   O^T [16 coordinates][8 rows] += V^T P^T, weights turned by movmatrix, values by byte permutes of the rows of two neighbouring keys
+//   output   O^T [16 coordinates][8 rows] += V^T P^T by m16n8k16 on fp16 numbers, weights turned by movmatrix, values by byte permutes of the rows of two neighbouring keys
 //
-// PARTS: fp16 numbers that stand for an fp32 query or weight.  2 keep 22 bits of each (results in fp32); 1 keeps 11 (results in bf16, which keep 8).  A row of queries is
-// multiplied by a power of two that brings its largest number to [2^10, 2^11), so nothing of weight gets too small for fp16; weights times their group's value scale are
-// relative to a kept scale (`vref`) for the same reason.
+// PARTS: fp16 numbers that stand for an fp32 query or weight.  2 keep 22 bits of each (results in fp32); 1 keeps 11 (results in bf16,
+// which keep 8).  A row of queries is multiplied by a power of two that brings its largest number to [2^10, 2^11), so nothing of weight gets too small for fp16; weights times
+// their group's value scale are relative to a kept scale (`vref`) for the same reason.
 //
-// Work: items (sequence, R rows, key head), cut into tiles of 128 positions, a warp 16 of them; all tiles of a call in one row, dealt evenly to the CTAs, so
+// Work: items (sequence, R rows, key head), cut into tiles of as many positions as the CTA's warps take at once; all tiles of a call in one row, dealt evenly to the CTAs, so
 // ragged batches and single long sequences fill the chip alike.  A CTA that has only a piece of an item leaves it in the workspace (the first or the last
-// of what it was dealt: two places), and kv8_join_kernel, a row a CTA, adds an item's pieces up in order.
+// of what it was dealt: two places), and kv8_join_kernel adds an item's pieces up in order.
+//
+// What bounds it: from some ten megabytes of codes on the bytes (32 sequences of 8,000 positions, 32 heads over 8 of 128: 62.7 us, 79 % of what a copy moves; of 32,000
+// 207 us, 95 %).  Below that what a launch has to do one after the other: look up what was dealt (1.3 us), queries and the first codes (2.5), the warps' sums (1.1), the join (3.5).
 #include <algorithm>
 #include <type_traits>
 
@@ -62,9 +66,10 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
 // P: numbers of a key and of a value, at most: 64, 128 or 256
 template <int CODE, int P, int NT, int PARTS> struct step_sizes {
     static constexpr int R = 8 * NT, KS = P / 16; // blocks of 16 value coordinates
-    // groups of 16 keys that a warp takes at once: two where the sums leave registers for them, which also gives the warp independent work.  Two CTAs of six warps an SM, or
-    // one of eight
-    static constexpr int min_ctas = P * NT <= 128 ? 2 : 1, W = min_ctas == 2 ? 6 : 8, U = P * NT <= 256 ? 2 : 1, threads = 32 * W, tile = 16 * W * U;
+    // groups of 16 keys that a warp takes at once: two where the sums leave registers for them, which also gives the warp independent work (32 sequences of 8,000 positions, 128
+    // numbers: 62.9 us, one 66.3; with two more drafted tokens each 94 and 107); with heads of 256, whose sums fill the registers, one (41 us, two 44).  Two CTAs of six warps
+    // an SM, or one of eight
+    static constexpr int min_ctas = P * NT <= 128 ? 2 : 1, W = min_ctas == 2 ? 6 : 8, U = P < 256 && P * NT <= 256 ? 2 : 1, threads = 32 * W, tile = 16 * W * U;
     // queries: int8 digits for steps of 32 numbers, or fp16 parts for steps of 16
     static constexpr bool digits = CODE == GGB_KV8_INT8;
     static constexpr int Q = digits ? PARTS + 2 : PARTS, QS = digits ? P / 32 : P / 16;
@@ -707,8 +712,9 @@ template <int CODE, int PARTS> int step_rows(const attn_args &a, int64_t max_new
     return rows <= 8 ? step_launch<CODE, 256, 1, PARTS>(a, max_new) : step_launch<CODE, 256, 2, PARTS>(a, max_new);
 }
 
-// sequences of many rows by the tiles' kernel, the others by the steps'
-constexpr int64_t kFew = 32;
+// sequences of many rows by the tiles' kernel, the others by the steps', which begin and end sooner.  16 sequences at 2,000 positions (bf16, 16 heads over 4 of 128), steps
+// against tiles: 64 rows 41 and 52 us, 96 rows 47 and 62, 128 rows 56 and 68; one sequence 17, 19, 19 and 22, 23, 25.  Beyond that tiles of 128 rows are not empty in part
+constexpr int64_t kFew = 128;
 template <int CODE, int PARTS> int attend(attn_args a, int64_t T, int64_t max_new) {
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
     const int64_t hpg = a.H / a.G;

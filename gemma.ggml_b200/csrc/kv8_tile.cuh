@@ -13,7 +13,13 @@
 // computes weights.  A maximum, and the value scale that weights are relative to, are kept until they are exceeded far enough (2^8 and 64 times), so the
 // output is hardly ever rescaled; the one is a row's, the other a group's, and no thread asks another.
 //
-// Work is dealt as in the steps' kernel: items (sequence, 128 rows, key head) of tiles in one row, an even share to every CTA, pieces of items joined behind.
+// Work is dealt as in the steps' kernel: items (sequence, 128 rows, key head) of tiles in one row, an even share to every CTA, pieces of items joined behind; where there are
+// many items, whole ones.
+//
+// What bounds it: nothing is full.  A tile takes a group about 2 us and both together 1: weights some 1,600 cycles a tile and group, products (queries and keys from shared
+// memory, which the code warps write at the same time) some 1,300 where 650 would do.  Beside that an item begins in 6 us (what was dealt, queries, the first codes) and ends in
+// 4 to 8 (sums, gate, pieces).  1,024 tokens behind 1,024, window 1,024, 16 heads over 4 of 128, bf16, gate: 38 us (230 TFLOP/s; 128 us by the steps' kernel); 4,096 tokens
+// from position 0: 202 us (340 TFLOP/s).
 #pragma once
 
 #include "kv8.cuh"
@@ -630,7 +636,9 @@ template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t m
     const int64_t groups = (max_new * hpg + kTileRows - 1) / kTileRows, items = (T * hpg + kTileRows - 1) / kTileRows * a.G;
     GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.positions + a.keep) / kTileKeys + kTileBegin + 2) < (1ll << 31), "kv8_attn: too many sequences, tokens, heads and positions for a launch");
     a.groups = (int)groups;
-    if (items >= 8 * ggb_sm_count()) a.part = nullptr;
+    // (bf16 results, 16 heads over 4 of 128, 4,096 tokens, 3.5 items an SM: whole 202 us, cut 223; 2,500 tokens in fp32, where what a chain leaves goes to memory and back, 187 and
+    // 172, 4,096 tokens 397 and 362)
+    if (items >= (PARTS == 1 ? 3 : 8) * ggb_sm_count()) a.part = nullptr;
     const size_t smem = std::max((size_t)tile_sizes(PARTS, a.D, a.Dv).smem, kOneCtaSmem);
     auto kfn = kv8_tile_kernel<CODE, PARTS>;
     const int rc = ggb_allow_smem(kfn, smem);
