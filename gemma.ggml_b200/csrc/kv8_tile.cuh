@@ -643,10 +643,9 @@ template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t m
     auto kfn = kv8_tile_kernel<CODE, PARTS>;
     const int rc = ggb_allow_smem(kfn, smem);
     if (rc) return rc;
-    static const int registers = [kfn] { // what the split takes has to be there, or it would be waited for without end
-        cudaFuncAttributes at{};
-        return cudaFuncGetAttributes(&at, kfn) == cudaSuccess ? at.numRegs : 0;
-    }();
+    cudaFuncAttributes built{}; // what the split takes has to be there, or it would be waited for without end
+    GGB_CUDA(cudaFuncGetAttributes(&built, kfn));
+    const int registers = built.numRegs;
     GGB_CHECK_ARG(registers * (kTileThreads / 128) >= kSoftWarps / 4 * kSoftRegs + kCodeWarps / 4 * kCodeRegs + kMmaRegs, "kv8_attn: built with %d registers a thread", registers);
     const unsigned ctas = (unsigned)(a.part ? std::min(kTileCtas, ggb_sm_count()) : ggb_sm_count());
     line_maps maps;
