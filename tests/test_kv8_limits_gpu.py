@@ -134,3 +134,47 @@ def test_fp32_results_over_many_positions(gpu, new):
     assert np.linalg.norm(got - want) < 3.7e-6 * np.linalg.norm(want)
     got = run_attention(gpu, F32, cache, q, new, starts, [12000], tables, new)
     assert np.linalg.norm(got - want) < 3.7e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("H", [33, 64, 128, 129, 256])
+def test_many_query_heads_of_one_key_head(gpu, dt, H):
+    r = np.random.default_rng(17)
+    new, pos = [1, 2, 0, 3], [90, 17, 4, 200]
+    starts, tables, pages = batch(r, new, pos, 48)
+    cache = P.Cache(P.E4M3, 1, 64, 80, 48, pages).filled(r)
+    poison(cache, tables, pos, new, True)
+    q = f32(r.standard_normal((6, H, 64)) * 0.2)
+    want, reach = P.attention(cache, q, starts, pos, np.maximum(tables, 0), 60, 3)
+    for scratch in (True, False):
+        check_attention(dt, run_attention(gpu, dt, cache, q, 8, starts, pos, tables, 3, 60, 3, scratch=scratch), want, reach, 64, 210)
+
+
+def test_the_first_call_of_a_process_may_be_captured(tmp_path):
+    """what a kernel asks of the driver once is asked for inside a capture"""
+    import subprocess
+    import sys
+    code = """
+import ctypes as C, sys
+sys.path[:0] = ["tests", "."]
+import numpy as np, gemma_ggml_b200 as G, kv8_plain as P
+from device_util import F32, dev, f32, from_dt, i32, zeros
+G.init()
+lib, r = G.cuda_lib(), np.random.default_rng(1)
+cache = P.Cache(P.INT8, 1, 64, 64, 64, 4).filled(r)
+q, n = f32(r.standard_normal((200, 2, 64)) * 0.2), int(lib.ggb_kv8_attn_scratch_bytes(64))
+b = [dev(G, q), dev(G, cache.pool), dev(G, i32([0, 1, 2, 3])), dev(G, i32([0, 200])), dev(G, i32([30])), zeros(G, 200 * 2 * 64 * 4), zeros(G, n)]
+G.sync()
+G.check(lib.ggb_capture_begin(), "capture")
+G.check(lib.ggb_op_kv8_attn(F32, P.INT8, b[0].ptr, b[1].ptr, b[2].ptr, 4, 64, 200, 200, 1, b[3].ptr, b[4].ptr, 2, 1, 64, 64, 0, 0, 0.0, None, None, 0, b[5].ptr, b[6].ptr, n), "kv8_attn")
+g = C.c_void_p()
+G.check(lib.ggb_capture_end(C.byref(g)), "capture")
+G.check(lib.ggb_graph_launch(g), "graph")
+G.sync()
+want, _ = P.attention(cache, q, [0, 200], [30], i32([[0, 1, 2, 3]]))
+got = from_dt(F32, b[5], (200, 2, 64))
+assert np.linalg.norm(got - want) < 5e-6 * np.linalg.norm(want)
+lib.ggb_graph_free(g)
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
