@@ -68,7 +68,8 @@ struct attn_args {
     void *out;
     int groups;     // items of a sequence and key head, at most
     int64_t rows_above, rows_up_to; // sequences of more rows (tokens x query heads of a key head) than the one, up to the other, are this kernel's
-    float *part;    // [CTA][2][rows][Dv + 2], or null: an item a CTA
+    float *part;    // pieces' sums [CTA][2][rows][Dv], or null: an item a CTA
+    float2 *part_ml; // their maxima and denominators [CTA][2][rows]
     int4 *desc;     // [CTA][2], of an item that begins or goes on here and ends elsewhere: sequence (or -1), rows, key head, first row; first and last CTA that have it, first token
     int vec_q, vec_out, vec_gate; // queries, results, rows of the gate begin on a 16-byte boundary
     int64_t positions; // that a page table has room for

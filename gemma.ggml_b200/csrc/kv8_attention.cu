@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
         if (lane == 0) svref[warp] = vref;
         __syncthreads();
         const bool whole_item = n == s_it.n;
-        float *part = a.part ? a.part + ((int64_t)blockIdx.x * 2 + (tile == 0)) * R * (a.Dv + 2) : nullptr;
+        const int64_t part_row = ((int64_t)blockIdx.x * 2 + (tile == 0)) * R;
         constexpr int TPR = Z::threads / R; // threads a row
         const int r = tid / TPR;
         if (r < s_it.rows) {
@@ -581,10 +581,10 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                     E *out = reinterpret_cast<E *>(a.out) + t * a.H * a.Dv + to;
                     out[0] = from_f32<E>(gated(a, y.x * end.f, t, to)), out[1] = from_f32<E>(gated(a, y.y * end.f, t, to + 1));
                 } else {
-                    *reinterpret_cast<float2 *>(part + (int64_t)r * (a.Dv + 2) + 2 * pr) = y;
+                    *reinterpret_cast<float2 *>(a.part + (part_row + r) * a.Dv + 2 * pr) = y;
                 }
             }
-            if (!whole_item && tid == r * TPR) part[(int64_t)r * (a.Dv + 2) + a.Dv] = M, part[(int64_t)r * (a.Dv + 2) + a.Dv + 1] = L;
+            if (!whole_item && tid == r * TPR) a.part_ml[part_row + r] = make_float2(M, L);
         }
         if (!whole_item && tile + n < s_it.n && tid == 0) { // joined by the CTAs that have it but for the last, whose own last piece may be another one's
             const piece &x = s_piece[slot];
@@ -613,17 +613,12 @@ template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_ker
     const int4 d = a.desc[2 * blockIdx.x], e = a.desc[2 * blockIdx.x + 1];
     if (d.x < 0) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hpg = a.H / a.G, b0 = e.x, pieces = e.y - b0 + 1, share = (blockIdx.x - b0) * gridDim.y + blockIdx.y, shares = (pieces - 1) * gridDim.y;
-    const int64_t pitch = a.Dv + 2;
     const int quads = a.Dv / 4, rows = d.y, q0 = rows * quads * share / shares, q1 = rows * quads * (share + 1) / shares, r0 = q0 / quads;
     if (q0 == q1) return;
     const int nq = min(256, q1 - q0), ways = 256 / nq, way = tid / nq;
-    auto piece = [&](int k, int r) { return a.part + (((int64_t)(b0 + k) * 2 + (k == 0)) * R + r) * pitch; };
+    auto piece = [&](int k, int r) { return ((int64_t)(b0 + k) * 2 + (k == 0)) * R + r; };
     float4 ahead[4];
-    auto load = [&](int k, int r, int c) {
-        const float2 *x = reinterpret_cast<const float2 *>(piece(k, r) + c);
-        const float2 p = x[0], s = x[1];
-        return make_float4(p.x, p.y, s.x, s.y);
-    };
+    auto load = [&](int k, int r, int c) { return *reinterpret_cast<const float4 *>(a.part + piece(k, r) * a.Dv + c); };
     int q = q0 + tid - way * nq;
 #pragma unroll
     for (int u = 0; u < 4; u++)
@@ -632,7 +627,7 @@ template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_ker
         float *f = s_f + (r - r0) * pieces, *g = s_g + (r - r0) * pieces, M = kNone, L = 0.f;
 #pragma unroll 8
         for (int k = lane; k < pieces; k += 32) {
-            const float2 ml = *reinterpret_cast<const float2 *>(piece(k, r) + a.Dv);
+            const float2 ml = a.part_ml[piece(k, r)];
             M = fmaxf(M, f[k] = ml.x);
             g[k] = ml.y;
         }
@@ -762,7 +757,8 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
     const int64_t positions = std::min<int64_t>(table_ld, (1ll << 31) / block_size) * block_size; // (they are 32-bit numbers)
     float *part = (float *)scratch;
     const attn_args a{q, (const uint8_t *)cache, tables, table_ld, block_size, n_seq, starts, pos0, H, G, D, Dv, window, window > 0 ? std::min<int64_t>(keep_first, positions) : 0, softcap, sink, gate, ldg,
-                      kv8_record(D, Dv, block_size), out, 0, 0, 0, part, part ? (int4 *)(part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2)) : nullptr, (uintptr_t)q % 16 == 0,
+                      kv8_record(D, Dv, block_size), out, 0, 0, 0, part, (float2 *)(part ? part + (size_t)kMaxCtas * 2 * kMaxRows * Dv : nullptr),
+                      (int4 *)(part ? part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2) : nullptr), (uintptr_t)q % 16 == 0,
                       (uintptr_t)out % 16 == 0, (uintptr_t)gate % 16 == 0 && ldg % 4 == 0, positions, ggb_wait_error_flag()};
     if (dt == GGB_TYPE_BF16) return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 1>(a, T, max_new) : attend<GGB_KV8_E4M3, 1>(a, T, max_new);
     return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 2>(a, T, max_new) : attend<GGB_KV8_E4M3, 2>(a, T, max_new);

@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
             const bool whole_item = n == it.n;
             const int row = it.row0 + r, tq = row / hpg, h = x.head * hpg + (row - tq * hpg);
             const int64_t t_row = it.t0 + tq;
-            float *part = whole_item ? nullptr : a.part + (((int64_t)blockIdx.x * 2 + (tile == 0)) * kTileRows + r) * (a.Dv + 2);
+            const int64_t part_row = ((int64_t)blockIdx.x * 2 + (tile == 0)) * kTileRows + r;
+            float *part = whole_item ? nullptr : a.part + part_row * a.Dv;
             float M = kNone, L = 0.f; // of the chains so far
             int k = grp;
             for (int upto = PARTS == 1 ? n : min(n, kChain);; upto = min(n, upto + kChain)) {
@@ -559,26 +560,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                         if (n > 1) v[u] = fmaf(__uint_as_float(o1[u]), f1, v[u]);
                     }
                     if (more) {
-                        if (!whole_item) {
-#pragma unroll
-                            for (int u = 0; u < 16; u += 2) {
-                                const float2 b = *reinterpret_cast<const float2 *>(part + 16 * cb + u);
-                                v[u] = fmaf(b.x, gb, v[u]), v[u + 1] = fmaf(b.y, gb, v[u + 1]);
-                            }
-                        } else if (a.vec_out) {
+                        const float *b = whole_item ? reinterpret_cast<const float *>(out) : part + 16 * cb;
+                        if (!whole_item || a.vec_out) {
 #pragma unroll
                             for (int u = 0; u < 16; u += 4) {
-                                const float4 b = *reinterpret_cast<const float4 *>(out + u);
-                                v[u] = fmaf(b.x, gb, v[u]), v[u + 1] = fmaf(b.y, gb, v[u + 1]), v[u + 2] = fmaf(b.z, gb, v[u + 2]), v[u + 3] = fmaf(b.w, gb, v[u + 3]);
+                                const float4 b4 = *reinterpret_cast<const float4 *>(b + u);
+                                v[u] = fmaf(b4.x, gb, v[u]), v[u + 1] = fmaf(b4.y, gb, v[u + 1]), v[u + 2] = fmaf(b4.z, gb, v[u + 2]), v[u + 3] = fmaf(b4.w, gb, v[u + 3]);
                             }
                         } else {
 #pragma unroll
-                            for (int u = 0; u < 16; u++) v[u] = fmaf(*reinterpret_cast<const float *>(out + u), gb, v[u]);
+                            for (int u = 0; u < 16; u++) v[u] = fmaf(b[u], gb, v[u]);
                         }
                     }
                     if (!whole_item) {
 #pragma unroll
-                        for (int u = 0; u < 16; u += 2) *reinterpret_cast<float2 *>(part + 16 * cb + u) = make_float2(v[u], v[u + 1]);
+                        for (int u = 0; u < 16; u += 4) *reinterpret_cast<float4 *>(part + 16 * cb + u) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
                         continue;
                     }
                     if (last) {
@@ -610,7 +606,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                 bar_sync(3, 32 * kSoftWarps);
                 tc_fence_after();
             }
-            if (!whole_item && grp == 0 && r < it.rows) *reinterpret_cast<float2 *>(part + a.Dv) = make_float2(M, L);
+            if (!whole_item && grp == 0 && r < it.rows) a.part_ml[part_row] = make_float2(M, L);
             if (!whole_item && tile + n < it.n && tid == 0) {
                 const deal d(s_all, gridDim.x);
                 a.desc[2 * blockIdx.x] = make_int4(it.s, it.rows, x.head, it.row0);
@@ -637,7 +633,7 @@ template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t m
     GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.positions + a.keep) / kTileKeys + kTileBegin + 2) < (1ll << 31), "kv8_attn: too many sequences, tokens, heads and positions for a launch");
     a.groups = (int)groups;
     // (bf16 results, 16 heads over 4 of 128, 4,096 tokens, 3.5 items an SM: whole 202 us, cut 223; 2,500 tokens in fp32, where what a chain leaves goes to memory and back, 187 and
-    // 172, 4,096 tokens 397 and 362)
+    // 164, 4,096 tokens 397 and 360)
     if (items >= (PARTS == 1 ? 3 : 8) * ggb_sm_count()) a.part = nullptr;
     const size_t smem = std::max((size_t)tile_sizes(PARTS, a.D, a.Dv).smem, kOneCtaSmem);
     auto kfn = kv8_tile_kernel<CODE, PARTS>;
