@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bars + T_Q_FULL);
+            warp_meet();
             bar_sync(3, 32 * kSoftWarps); // the rows' factors
             if (tid == 32 * kSoftWarps - 1) { // while the first scores are under way: the piece behind this one
                 piece y = x;
@@ -483,7 +484,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                         vref = most_v, vinv = 1.f / most_v;
                     }
                     // (from here on the weights that this tile's go over have been read, and the output that they went into is there: tile k - 2's products)
-                    if (k >= 2 && !wait_long(bars + T_V_FREE + 8 * grp, (ph + (k >> 1) - 1) & 1, dead)) lost = true;
+                    // Rows that grew have parted the lanes; the wait's vote joins them, as loads and stores of tensor memory ask for
+                    if (k >= 2) {
+                        if (!wait_long(bars + T_V_FREE + 8 * grp, (ph + (k >> 1) - 1) & 1, dead)) lost = true;
+                    } else {
+                        warp_meet();
+                    }
                     tc_fence_after();
                     if ((PARTS == 1 ? k : k % kChain) >= 2 && __any_sync(0xffffffffu, over != 1.f)) {
 #pragma unroll 1
@@ -549,6 +555,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
 #pragma unroll
                         for (int u = 0; u < 4; u++) gt[u] = a.vec_gate ? *reinterpret_cast<const float4 *>(gate + 4 * u) : make_float4(gate[4 * u], gate[4 * u + 1], gate[4 * u + 2], gate[4 * u + 3]);
                     uint32_t o0[16], o1[16];
+                    warp_meet(); // lanes whose rows end ahead of the others go on alone, here and in the round before
                     tmem_load16(tmem + lanes + kOutCol + 16 * cb, o0);
                     if (n > 1) tmem_load16(tmem + lanes + kOutCol + a.Dv + 16 * cb, o1);
                     if (r >= it.rows) continue;
@@ -603,6 +610,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                 if (last) break;
                 l = 0.f, m = kNone, vref = 0.f;
                 tc_fence_before(); // the next chain begins when the other group has read this one's too
+                warp_meet();
                 bar_sync(3, 32 * kSoftWarps);
                 tc_fence_after();
             }

@@ -178,3 +178,19 @@ lib.ggb_graph_free(g)
 """
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("new,Dv", [([129], 128), ([143, 161], 112), ([190, 130], 48)])
+def test_portions_whose_last_rows_end_inside_a_warp(gpu, dt, new, Dv):
+    """rows that end ahead of a warp's others, which go on alone through the output's columns, and rows that see nothing of a tile that others see"""
+    r = np.random.default_rng(18)
+    pos = [5, 40][:len(new)]
+    starts, tables, pages = batch(r, new, pos, 32)
+    cache = P.Cache(P.INT8, 1, 64, Dv, 32, pages).filled(r)
+    poison(cache, tables, pos, new, True)
+    n = int(starts[-1])
+    q, gate = f32(r.standard_normal((n, 1, 64)) * 0.2), f32(r.standard_normal((n, 1, Dv)))
+    want, reach = P.attention(cache, q, starts, pos, np.maximum(tables, 0), 33, 2, gate=gate)
+    for scratch in (True, False):
+        check_attention(dt, run_attention(gpu, dt, cache, q, n, starts, pos, tables, max(new), 33, 2, gate=gate, scratch=scratch), want, reach, 64, 240)
