@@ -114,6 +114,17 @@ __device__ __forceinline__ float gated(const attn_args &a, float y, int64_t t, i
 
 constexpr float kNone = -3e38f; // a maximum of nothing: a number, so that the differences to it are
 
+// What goes into the products with the codes is 2^(s - m) times the group's value scale, as fp16 numbers.  These have 11 bits above 2^-14 and lose them below, so the products
+// are brought to the upper part of the range: each row keeps a power of two 2^d that its products are multiplied by, such that the largest one that it has met (of what it
+// sees: a scale says nothing without a weight) was at 2^kNewWeight when it was found, and lets it grow to 2^kMostWeight.  Any other is off by its last
+// bit or by half of fp16's smallest step, 2^-25, which is 2^-32 of that.  Maxima are whole numbers, so 2^d stays what it is when they move.  The denominator is a sum of its own,
+// of 2^(s - m).  (Relative to the largest scale of a tile instead, seen or not, a row whose own values are 10^5 times smaller came out 2 % off, 10^8 times: zero.)
+constexpr int kNewWeight = 7, kMostWeight = 15;
+// a whole number that a scale's logarithm is below; not below -110, so that d stays one that 2^d exists of
+__device__ __forceinline__ int scale_exponent(float v) { return max((int)(__float_as_uint(v) >> 23) - 126, -110); }
+// v 2^d, |d| <= 126; a number where it is beyond all of them (the scale of a group whose weights are nothing)
+__device__ __forceinline__ float scale_times(float v, int d) { return fminf(v * __uint_as_float((uint32_t)(127 + d) << 23), 3e38f); }
+
 // the rows of an item and the tiles that they see: [0, n_keep) in kt tiles, then [lo, i1] in tiles from position TILE * w0 on
 struct item {
     int s, rg, row0, rows; // rows [row0, row0 + rows) of the sequence: its tokens x the query heads of a key head

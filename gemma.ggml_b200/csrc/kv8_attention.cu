@@ -13,8 +13,8 @@
 //   output   O^T [16 coordinates][8 rows] += V^T P^T by m16n8k16 on fp16 numbers, weights turned by movmatrix, values by byte permutes of the rows of two neighbouring keys
 //
 // PARTS: fp16 numbers that stand for an fp32 query or weight.  2 keep 22 bits of each (results in fp32); 1 keeps 11 (results in bf16,
-// which keep 8).  A row of queries is multiplied by a power of two that brings its largest number to [2^10, 2^11), so nothing of weight gets too small for fp16; weights times
-// their group's value scale are relative to a kept scale (`vref`) for the same reason.
+// which keep 8).  A row of queries is multiplied by a power of two that brings its largest number to [2^10, 2^11), so nothing of weight gets too small for fp16; so are a row's
+// weights times their groups' value scales (kv8.cuh).
 //
 // Work: items (sequence, R rows, key head), cut into tiles of as many positions as the CTA's warps take at once; all tiles of a call in one row, dealt evenly to the CTAs, so
 // ragged batches and single long sequences fill the chip alike.  A CTA that has only a piece of an item leaves it in the workspace (the first or the last
@@ -79,7 +79,7 @@ template <int CODE, int P, int NT, int PARTS> struct step_sizes {
     static constexpr int S = P == 256 ? (NT == 1 ? 2 : 3) : P == 128 ? (NT == 1 ? 4 : NT == 2 ? 4 : 2) : NT == 4 ? 7 : 4;
     static constexpr size_t q_bytes = (size_t)Q * NT * QS * 256, ring_bytes = (size_t)W * S * stage, red_bytes = (size_t)W * R * P * 4;
     static_assert((beside || red_bytes <= ring_bytes) && stage % 1024 == 0, "shared memory");
-    static constexpr size_t smem = 1024 + q_bytes + ring_bytes + (beside ? red_bytes : 0) + (size_t)W * (R * 8 + 768) + R * 8 + 64;
+    static constexpr size_t smem = 1024 + q_bytes + ring_bytes + (beside ? red_bytes : 0) + (size_t)W * (R * 12 + 768) + R * 8 + 64;
     static_assert((smem + 2048) * min_ctas <= 227 * 1024, "shared memory of an SM");
 };
 // where the pair of coordinates 2 i, 2 i + 1 of the 16 (P = 64: 8) numbers of lane group g lies in its row of the reduction, in pairs: rows of a warp's stores in different banks
@@ -165,10 +165,9 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, c4 = lane & 3;
     int2 *lines = reinterpret_cast<int2 *>(base_at + Z::ring_bytes + Z::q_bytes) + warp * 96; // [32]: lines of the tiles' keys and values
     float2 *scales = reinterpret_cast<float2 *>(lines + 32);                                  // [64]
-    float *sm = reinterpret_cast<float *>(base_at + Z::ring_bytes + Z::q_bytes + Z::W * 768), *sl = sm + Z::W * R, *srow = sl + Z::W * R;
+    float *sm = reinterpret_cast<float *>(base_at + Z::ring_bytes + Z::q_bytes + Z::W * 768), *sl = sm + Z::W * R, *sd = sl + Z::W * R, *srow = sd + Z::W * R;
     int *spos = reinterpret_cast<int *>(srow + R);
-    float *svref = reinterpret_cast<float *>(spos + R);
-    float2 *red = reinterpret_cast<float2 *>(base_at + (Z::beside ? Z::ring_bytes + Z::q_bytes + Z::W * (768 + R * 8) + R * 8 + 64 : 0));
+    float2 *red = reinterpret_cast<float2 *>(base_at + (Z::beside ? Z::ring_bytes + Z::q_bytes + Z::W * (768 + R * 12) + R * 8 + 64 : 0));
     const uint32_t ring = ring0 + warp * Z::S * Z::stage, bars = smem_u32(s_bars) + 8 * warp * Z::S;
     if (lane == 0)
         for (int k = 0; k < Z::S; k++) mbar_init(bars + 8 * k, 1);
@@ -328,11 +327,12 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
         const int up = s_it.i0 - last_of - 16 * Z::U * warp, down = max(s_it.lo, a.window > 0 ? (int)max((int64_t)0, s_it.i1 - a.window + 1) : 0) - 16 * Z::U * warp;
         const int whole0 = s_it.kt + max(0, (down + Z::tile - 1) / Z::tile - s_it.w0), wholes = up < 0 ? 0 : max(0, s_it.kt + up / Z::tile - s_it.w0 - whole0 + 1);
 
-        float rowf[NT][2], m[NT][2], l[NT][2], o[KS][NT][4], vref = 0.f, vinv = 0.f;
+        float rowf[NT][2], m[NT][2], l[NT][2], o[KS][NT][4];
+        int pow[NT][2]; // products of weights and scales are taken times 2^pow
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) rowf[t][e] = srow[8 * t + 2 * c4 + e], m[t][e] = kNone, l[t][e] = 0.f;
+            for (int e = 0; e < 2; e++) rowf[t][e] = srow[8 * t + 2 * c4 + e], m[t][e] = kNone, l[t][e] = 0.f, pow[t][e] = 0;
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
@@ -440,46 +440,53 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                 }
             }
             // ---- weights
-            float vmost = sc[0].y;
             bool grow = false;
+            int lv[Z::U];
 #pragma unroll
             for (int u = 0; u < Z::U; u++) {
-                vmost = fmaxf(vmost, sc[u].y);
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) grow |= z[u][t][e] > m[t][e & 1] + 8.f;
-            }
-            if (__any_sync(0xffffffffu, grow || vmost > 64.f * vref)) {
-                const float vnew = vmost > 64.f * vref ? vmost : vref, vf = vnew > 0.f ? vref / vnew : 0.f;
-                vref = vnew, vinv = vnew > 0.f ? 1.f / vnew : 0.f;
+                lv[u] = scale_exponent(sc[u].y);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float x = fmaxf(fmaxf(z[0][t][e], z[0][t][e + 2]), fmaxf(z[Z::U - 1][t][e], z[Z::U - 1][t][e + 2]));
+                        const float most = m[t][e] + (float)min(8, kMostWeight - lv[u] - pow[t][e]);
+                        grow |= z[u][t][e] > most || z[u][t][e + 2] > most;
+                    }
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float x = kNone, p = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < Z::U; u++) x = fmaxf(x, fmaxf(z[u][t][e], z[u][t][e + 2]));
 #pragma unroll
                         for (int off = 4; off <= 16; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                        x = fmaxf(x, m[t][e]);
-                        const float f = exp2f(m[t][e] - x);
-                        m[t][e] = x;
-                        l[t][e] *= f;
+                        x = fmaxf(ceilf(x), m[t][e]);
 #pragma unroll
-                        for (int i = 0; i < KS; i++) o[i][t][e] *= f * vf, o[i][t][e + 2] *= f * vf;
+                        for (int u = 0; u < Z::U; u++) p = fmaxf(p, (fmaxf(z[u][t][e], z[u][t][e + 2]) - x) + (float)lv[u]);
+#pragma unroll
+                        for (int off = 4; off <= 16; off <<= 1) p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, off));
+                        const float d2 = (float)pow[t][e] + (x - m[t][e]), d = fminf(d2, (float)kNewWeight - ceilf(p)), f = exp2f(d - d2);
+                        l[t][e] *= exp2f(m[t][e] - x);
+                        m[t][e] = x, pow[t][e] = (int)d;
+#pragma unroll
+                        for (int i = 0; i < KS; i++) o[i][t][e] *= f, o[i][t][e + 2] *= f;
                     }
             }
             uint32_t pb[Z::U][PARTS][NT][2];
 #pragma unroll
             for (int u = 0; u < Z::U; u++) {
-                const float vrel = sc[u].y * vinv;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
+                    const float vrel[2] = {scale_times(sc[u].y, pow[t][0]), scale_times(sc[u].y, pow[t][1])};
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         w[e] = ex2_approx(z[u][t][e] - m[t][e & 1]);
                         l[t][e & 1] += w[e];
-                        w[e] *= vrel;
+                        w[e] *= vrel[e & 1];
                     }
 #pragma unroll
                     for (int y = 0; y < 2; y++) {
@@ -543,12 +550,11 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                 const int r = 8 * t + 2 * c4 + e;
 #pragma unroll
                 for (int off = 4; off <= 16; off <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], off);
-                if (g8 == 0) sm[warp * R + r] = m[t][e], sl[warp * R + r] = l[t][e];
+                if (g8 == 0) sm[warp * R + r] = m[t][e], sl[warp * R + r] = l[t][e], sd[warp * R + r] = (float)pow[t][e];
                 float2 *row = red + (warp * R + r) * (P / 2);
 #pragma unroll
                 for (int i = 0; i < KS; i++) row[64 * (i / 8) + red_at<P>(g8, i % 8, c4)] = make_float2(o[i][t][e], o[i][t][e + 2]);
             }
-        if (lane == 0) svref[warp] = vref;
         __syncthreads();
         const bool whole_item = n == s_it.n;
         const int64_t part_row = ((int64_t)blockIdx.x * 2 + (tile == 0)) * R;
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
             for (int w = 0; w < Z::W; w++) {
                 f[w] = exp2f(sm[w * R + r] - M);
                 L = fmaf(sl[w * R + r], f[w], L);
-                f[w] *= svref[w];
+                f[w] = exp2f((sm[w * R + r] - M) - sd[w * R + r]);
             }
             const int row = s_it.row0 + r, tq = row / hpg, h = s_piece[slot].head * hpg + (row - tq * hpg);
             const int64_t t = s_it.t0 + tq;

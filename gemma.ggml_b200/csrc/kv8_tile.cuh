@@ -6,12 +6,12 @@
 //            tensor cores want them
 //   scores   S [128][64] = (q_l + q_h) K^T: queries as PARTS fp16 numbers, rows by a power of two in the upper part of the range (as in the steps' kernel)
 //   weights  a thread a row: S from tensor memory times the group's key scale and the row's factor, soft cap, mask, 2^(s - m), times the group's value
-//            scale over a kept one, as PARTS fp16 numbers back to tensor memory, over the scores
+//            scale, as PARTS fp16 numbers in the upper part of the range back to tensor memory, over the scores
 //   output   O [128][Dv] += (p_l + p_h) V, weights from tensor memory, the values as they lie (MN-major B)
 //
 // Two groups of four warps take the tiles alternately, each with scores, maxima, sums and output of its own, so that the tensor cores work for the one while the other
-// computes weights.  A maximum, and the value scale that weights are relative to, are kept until they are exceeded far enough (2^8 and 64 times), so the
-// output is hardly ever rescaled; the one is a row's, the other a group's, and no thread asks another.
+// computes weights.  A maximum, and the largest product of a weight and a scale that the row has met, are kept until they are exceeded by 2^8, so the
+// output is hardly ever rescaled; both are a row's, and no thread asks another.
 //
 // Work is dealt as in the steps' kernel: items (sequence, 128 rows, key head) of tiles in one row, an even share to every CTA, pieces of items joined behind; where there are
 // many items, whole ones.
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
             const int lo_last = a.window > 0 ? (int)max((int64_t)0, it.i1 - a.window + 1) : 0, whole_from = max(it.lo, lo_last), ph = grp ? ph1 : ph0;
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, ts = tmem + lanes + kScoreCol + grp * 64, tw = tmem + lanes + kWeightCol + grp * 64, to = tmem + lanes + kOutCol + grp * a.Dv;
             const float rowf = srow[r], cap = a.cap * kLog2e, inv_cap = a.cap > 0.f ? kLn2 / a.cap : 0.f;
-            float m = kNone, l = 0.f, vref = 0.f, vinv = 0.f;
+            float m = kNone, l = 0.f, d = 0.f; // weights are relative to 2^m, their products with values' scales to 2^(m - d)
             bool lost = false;
             const bool whole_item = n == it.n;
             const int row = it.row0 + r, tq = row / hpg, h = x.head * hpg + (row - tq * hpg);
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                     const float4 *sc4 = reinterpret_cast<const float4 *>(scales + ((ph0 + ph1 + k) & 15) * 4);
                     const float4 sa = sc4[0], sb = sc4[1];
                     const float ks[4] = {sa.x, sa.z, sb.x, sb.z}, vs[4] = {sa.y, sa.w, sb.y, sb.w};
-                    float y[4][16], f[4], mx = kNone;
+                    float y[4][16], f[4], top[4];
                     tmem_load32(ts, reinterpret_cast<uint32_t *>(y[0]));
                     tmem_load32(ts + 32, reinterpret_cast<uint32_t *>(y[2]));
                     tc_fence_before();
@@ -471,17 +471,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                         float big[2] = {y[g][0], y[g][1]};
 #pragma unroll
                         for (int c = 2; c < 16; c++) big[c & 1] = fmaxf(big[c & 1], y[g][c]);
-                        mx = fmaxf(mx, fmaxf(big[0], big[1]) * f[g]);
+                        top[g] = fmaxf(big[0], big[1]) * f[g];
                     }
-                    float over = 1.f;
-                    if (mx > m + 8.f) {
-                        over = exp2f(m - mx);
-                        m = mx, l *= over;
-                    }
-                    const float most_v = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-                    if (most_v > 64.f * vref) {
-                        over *= vref / most_v;
-                        vref = most_v, vinv = 1.f / most_v;
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), m2 = mx > m + 8.f ? ceilf(mx) : m;
+                    float pm = -INFINITY, over = 1.f; // the largest product of a weight and a scale, in powers of two: only what the row sees counts
+#pragma unroll
+                    for (int g = 0; g < 4; g++) pm = fmaxf(pm, (top[g] - m2) + (float)scale_exponent(vs[g]));
+                    const float d2 = d + (m2 - m);
+                    if (m2 != m || pm + d2 > (float)kMostWeight) {
+                        l *= exp2f(m - m2), m = m2;
+                        d = fminf(d2, (float)kNewWeight - ceilf(pm));
+                        over = exp2f(d - d2);
                     }
                     // (from here on the weights that this tile's go over have been read, and the output that they went into is there: tile k - 2's products)
                     // Rows that grew have parted the lanes; the wait's vote joins them, as loads and stores of tensor memory ask for
@@ -504,9 +504,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
 #pragma unroll
                     for (int g = 0; g < 4; g++) {
                         f32x2 sum[2] = {0, 0};
-                        const float rel = vs[g] > 0.f ? fmaxf(vs[g] * vinv, 0x1p-40f) : 1.f; // (a scale of zero: values of zero.  2^-40 of another value's scale: nothing)
-                        // one part: the scale goes with the exponent, and out of the sum again
-                        const float power = PARTS == 1 ? lg2_approx(rel) : 0.f, shift = power - m;
+                        const float rel = PARTS == 1 ? 0.f : scale_times(vs[g], (int)d);
+                        // one part: the scale goes with the exponent, and out of the sum again (2^-60: below every 16-bit number, and the weight of the sum still there)
+                        const float power = PARTS == 1 ? fmaxf(lg2_approx(vs[g]) + d, -60.f) : 0.f, shift = power - m;
                         uint32_t hi[8], lo2[8];
 #pragma unroll
                         for (int c = 0; c < 8; c++) {
@@ -538,13 +538,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                 else wait_long(bars + T_V_FREE + 8 * grp, (ph + ((k - 2) >> 1)) & 1, dead);
                 tc_fence_after();
                 bar_sync(3, 32 * kSoftWarps); // the tables are no longer read
-                st[3 * grp * kTileRows + r] = l, st[(3 * grp + 1) * kTileRows + r] = m, st[(3 * grp + 2) * kTileRows + r] = vref;
+                st[3 * grp * kTileRows + r] = l, st[(3 * grp + 1) * kTileRows + r] = m, st[(3 * grp + 2) * kTileRows + r] = d;
                 bar_sync(3, 32 * kSoftWarps);
                 const float before = M, m0 = st[kTileRows + r], m1 = n > 1 ? st[4 * kTileRows + r] : kNone;
                 M = fmaxf(fmaxf(m0, m1), before);
                 const float g0 = exp2f(m0 - M), g1 = n > 1 ? exp2f(m1 - M) : 0.f, gb = more ? exp2f(before - M) : 0.f;
                 L = fmaf(st[r], g0, n > 1 ? st[3 * kTileRows + r] * g1 : 0.f) + (more ? L * gb : 0.f);
-                const float f0 = g0 * st[2 * kTileRows + r], f1 = g1 * st[5 * kTileRows + r];
+                const float f0 = exp2f((m0 - M) - st[2 * kTileRows + r]), f1 = n > 1 ? exp2f((m1 - M) - st[5 * kTileRows + r]) : 0.f;
                 const row_end end(a, r < it.rows ? h : 0, M, L);
 #pragma unroll 1
                 for (int cb = grp; cb < a.Dv / 16; cb += 2) {
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                     }
                 }
                 if (last) break;
-                l = 0.f, m = kNone, vref = 0.f;
+                l = 0.f, m = kNone, d = 0.f;
                 tc_fence_before(); // the next chain begins when the other group has read this one's too
                 warp_meet();
                 bar_sync(3, 32 * kSoftWarps);
