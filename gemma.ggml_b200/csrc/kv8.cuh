@@ -112,6 +112,7 @@ struct row_end {
 };
 __device__ __forceinline__ float gated(const attn_args &a, float y, int64_t t, int64_t at) { return a.gate ? y / (1.f + expf(-a.gate[t * a.ldg + at])) : y; }
 
+constexpr int kQueryParts = 2; // fp16 numbers that stand for an fp32 query: 22 bits
 constexpr float kNone = -3e38f; // a maximum of nothing: a number, so that the differences to it are
 
 // What goes into the products with the codes is 2^(s - m) times the group's value scale, as fp16 numbers.  These have 11 bits above 2^-14 and lose them below, so the products

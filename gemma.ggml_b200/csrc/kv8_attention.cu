@@ -12,8 +12,9 @@
 //   weights  in the registers that the scores are in: 2^(s - m); a kept maximum is followed only when a score exceeds it by 8 (a vote, no shuffles otherwise)
 //   output   O^T [16 coordinates][8 rows] += V^T P^T by m16n8k16 on fp16 numbers, weights turned by movmatrix, values by byte permutes of the rows of two neighbouring keys
 //
-// PARTS: fp16 numbers that stand for an fp32 query or weight.  2 keep 22 bits of each (results in fp32); 1 keeps 11 (results in bf16,
-// which keep 8).  A row of queries is multiplied by a power of two that brings its largest number to [2^10, 2^11), so nothing of weight gets too small for fp16; so are a row's
+// PARTS: fp16 numbers that stand for an fp32 weight.  2 keep 22 bits of it (results in fp32); 1 keeps 11 (results in bf16,
+// which keep 8).  Queries are two (or digits) for either: what is cut off them a score multiplies, by 40 where two scores of 40 are weighed against one another, and 11 bits then
+// left results 2 % off.  A row of queries is multiplied by a power of two that brings its largest number to [2^10, 2^11), so nothing of weight gets too small for fp16; so are a row's
 // weights times their groups' value scales (kv8.cuh).
 //
 // Work: items (sequence, R rows, key head), cut into tiles of as many positions as the CTA's warps take at once; all tiles of a call in one row, dealt evenly to the CTAs, so
@@ -72,7 +73,7 @@ template <int CODE, int P, int NT, int PARTS> struct step_sizes {
     static constexpr int min_ctas = P * NT <= 128 ? 2 : 1, W = min_ctas == 2 ? 6 : 8, U = P < 256 && P * NT <= 256 ? 2 : 1, threads = 32 * W, tile = 16 * W * U;
     // queries: int8 digits for steps of 32 numbers, or fp16 parts for steps of 16
     static constexpr bool digits = CODE == GGB_KV8_INT8;
-    static constexpr int Q = digits ? PARTS + 2 : PARTS, QS = digits ? P / 32 : P / 16;
+    static constexpr int Q = digits ? PARTS + 2 : kQueryParts, QS = digits ? P / 32 : P / 16;
     static constexpr int half = 16 * P, stage = 2 * half; // a group's keys, then their values; S of them on their way or in use
     // the warps' sums of a piece meet beside the stages, on which the next piece's codes are arriving (16 rows of 256: no room, over them)
     static constexpr bool beside = P == 64 || (P == 128 && NT > 1) || (P == 256 && NT == 1);
@@ -138,11 +139,9 @@ template <int CODE, int P, int NT, int PARTS> __device__ __forceinline__ void st
             uint2 p = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
             const int step = 4 * (d / 64) + (d % 16) / 4;
             sq[(t * Z::QS + step) * 32 + to] = p;
-            if (PARTS == 2) {
-                const float2 b0 = half2_floats(p.x), b1 = half2_floats(p.y);
-                p = make_uint2(half2_bits(y[0] - b0.x, y[1] - b0.y), half2_bits(y[2] - b1.x, y[3] - b1.y));
-                sq[((NT + t) * Z::QS + step) * 32 + to] = p;
-            }
+            const float2 b0 = half2_floats(p.x), b1 = half2_floats(p.y);
+            p = make_uint2(half2_bits(y[0] - b0.x, y[1] - b0.y), half2_bits(y[2] - b1.x, y[3] - b1.y));
+            sq[((NT + t) * Z::QS + step) * 32 + to] = p;
         }
     }
 }
@@ -389,11 +388,11 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                             halves_of<CODE>(w0[w], a0, a2);
                             halves_of<CODE>(w1[w], a1, a3);
 #pragma unroll
-                            for (int part = PARTS - 1; part >= 0; part--)
+                            for (int part = Z::Q - 1; part >= 0; part--)
 #pragma unroll
                                 for (int t = 0; t < NT; t++) {
                                     const uint2 y = sq[((part * NT + t) * Z::QS + 4 * b + w) * 32 + lane];
-                                    if (b + w == 0 && part == PARTS - 1) mma16816_first(z[u][t], a0, a1, a2, a3, y.x, y.y);
+                                    if (b + w == 0 && part == Z::Q - 1) mma16816_first(z[u][t], a0, a1, a2, a3, y.x, y.y);
                                     else mma16816(z[u][t], a0, a1, a2, a3, y.x, y.y);
                                 }
                         }

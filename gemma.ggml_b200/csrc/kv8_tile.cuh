@@ -4,7 +4,7 @@
 //
 //   codes    copied by TMA (one warp asks) three tiles ahead; four warps for keys and four for values, 16 positions each, turn them into fp16 (exactly) and lay them out as the
 //            tensor cores want them
-//   scores   S [128][64] = (q_l + q_h) K^T: queries as PARTS fp16 numbers, rows by a power of two in the upper part of the range (as in the steps' kernel)
+//   scores   S [128][64] = (q_l + q_h) K^T: queries as two fp16 numbers, rows by a power of two in the upper part of the range (as in the steps' kernel)
 //   weights  a thread a row: S from tensor memory times the group's key scale and the row's factor, soft cap, mask, 2^(s - m), times the group's value
 //            scale, as PARTS fp16 numbers in the upper part of the range back to tensor memory, over the scores
 //   output   O [128][Dv] += (p_l + p_h) V, weights from tensor memory, the values as they lie (MN-major B)
@@ -60,9 +60,9 @@ template <int N> __device__ __forceinline__ void fewer_registers() { asm volatil
 
 struct tile_sizes {
     uint32_t q, k, v, raw, raw_stage, stats, scales, tables, bars, smem; // byte offsets behind the 1024-byte boundary, and bytes in all
-    __host__ __device__ tile_sizes(int parts, int D, int Dv) {
+    __host__ __device__ tile_sizes(int D, int Dv) {
         const uint32_t D64 = (D + 63) / 64, V64 = (Dv + 63) / 64;
-        q = 0, k = parts * D64 * kTileRows * 128, v = k + 2 * D64 * kTileKeys * 128, raw = v + 2 * V64 * kTileKeys * 128;
+        q = 0, k = kQueryParts * D64 * kTileRows * 128, v = k + 2 * D64 * kTileKeys * 128, raw = v + 2 * V64 * kTileKeys * 128;
         raw_stage = 4096 * (D64 + V64); // a tile's four groups of keys, then of values, as they are copied
         stats = raw + kAhead * raw_stage;
         scales = stats + 7 * kTileRows * 4, tables = scales + 16 * 4 * 8, bars = tables + 256, smem = 1024 + bars + 256;
@@ -85,14 +85,14 @@ template <int PARTS, int KS> __device__ __forceinline__ void tile_products(const
         mbar_wait_bounded(m.bars + T_K_FULL + 8 * s, par, m.dead);
         tc_fence_after();
 #pragma unroll
-        for (int part = PARTS - 1; part >= 0; part--) { // the small part first
+        for (int part = kQueryParts - 1; part >= 0; part--) { // the small part first
             const uint32_t ql = q_lo + part * (m.q_part >> 4);
             if (KS > 0) {
 #pragma unroll
-                for (int b = 0; b < KS / 4; b++) umma_ss_k4(d, ql + b * (kTileRows * 8), kl + b * (kTileKeys * 8), id_s, part < PARTS - 1 || b > 0);
+                for (int b = 0; b < KS / 4; b++) umma_ss_k4(d, ql + b * (kTileRows * 8), kl + b * (kTileKeys * 8), id_s, part < kQueryParts - 1 || b > 0);
             } else {
                 for (int k = 0; k < m.ksteps; k++)
-                    umma_ss(d, ql + (k >> 2) * (kTileRows * 8) + 2 * (k & 3), kl + (k >> 2) * (kTileKeys * 8) + 2 * (k & 3), id_s, part < PARTS - 1 || k > 0);
+                    umma_ss(d, ql + (k >> 2) * (kTileRows * 8) + 2 * (k & 3), kl + (k >> 2) * (kTileKeys * 8) + 2 * (k & 3), id_s, part < kQueryParts - 1 || k > 0);
             }
         }
         umma_arrive(m.bars + T_S_FULL + 8 * s);
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
     __shared__ unsigned s_scan[kTileThreads / 32], s_end, s_all;
     const uint32_t raw0 = smem_u32(kt_raw), base = (raw0 + 1023u) & ~1023u;
     uint8_t *gbase = kt_raw + (base - raw0);
-    const tile_sizes z(PARTS, a.D, a.Dv);
+    const tile_sizes z(a.D, a.Dv);
     const uint32_t bars = base + z.bars;
     volatile int *dead = reinterpret_cast<volatile int *>(gbase + z.bars + T_DEAD);
     float *st = reinterpret_cast<float *>(gbase + z.stats);
@@ -394,11 +394,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
                     uint2 p = make_uint2(half2_bits(y[0], y[1]), half2_bits(y[2], y[3]));
                     const uint32_t at = base + z.q + (u >> 2) * (kTileRows * 128) + r * 128 + (((2 * (u & 3) + (part >> 1)) ^ (r & 7)) << 4) + (part & 1) * 8;
                     asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(p.x), "r"(p.y) : "memory");
-                    if (PARTS == 2) {
-                        const float2 b0 = half2_floats(p.x), b1 = half2_floats(p.y);
-                        p = make_uint2(half2_bits(y[0] - b0.x, y[1] - b0.y), half2_bits(y[2] - b1.x, y[3] - b1.y));
-                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + q_part), "r"(p.x), "r"(p.y) : "memory");
-                    }
+                    const float2 b0 = half2_floats(p.x), b1 = half2_floats(p.y);
+                    p = make_uint2(half2_bits(y[0] - b0.x, y[1] - b0.y), half2_bits(y[2] - b1.x, y[3] - b1.y));
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + q_part), "r"(p.x), "r"(p.y) : "memory");
                 }
             }
             fence_async_smem();
@@ -643,7 +641,7 @@ template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t m
     // (bf16 results, 16 heads over 4 of 128, 4,096 tokens, 3.5 items an SM: whole 202 us, cut 223; 2,500 tokens in fp32, where what a chain leaves goes to memory and back, 187 and
     // 164, 4,096 tokens 397 and 360)
     if (items >= (PARTS == 1 ? 3 : 8) * ggb_sm_count()) a.part = nullptr;
-    const size_t smem = std::max((size_t)tile_sizes(PARTS, a.D, a.Dv).smem, kOneCtaSmem);
+    const size_t smem = std::max((size_t)tile_sizes(a.D, a.Dv).smem, kOneCtaSmem);
     auto kfn = kv8_tile_kernel<CODE, PARTS>;
     const int rc = ggb_allow_smem(kfn, smem);
     if (rc) return rc;

@@ -5,7 +5,8 @@ sum_j w_j, s_j the scale of the group that value j lies in and top the largest c
 
 Bounds, u = 2^-24.  A score is off by at most (D + 8) u S (S: the largest sum of |q_d k_d| of the row), a weight by that and so is the denominator; sums of n terms by n u; 64 u for what is
 rounded a few times each.  Weights go to the products as 16-bit numbers: one of 11 bits for bf16 results, 2^-11 of itself (a rounding is off by half a step), two for fp32 results, 2^-22; and,
-being numbers of a smallest step, each by no more than 2^-32 of the largest product of a weight and a scale of its row: together n 2^-32 R.  With bf16 results queries may be rounded to 11 bits, too, and the result is off by 2^-8 of itself.
+being numbers of a smallest step, each by no more than 2^-32 of the largest product of a weight and a scale of its row: together n 2^-32 R.  With bf16 results queries may be rounded to steps of 2^-20 of their row's largest (a score
+by 2^-20 Q, Q the largest sum of |k_d| times that), and the result is off by 2^-8 of itself.
 Nothing else: no bound counts a value that the row does not see, or does not weigh."""
 import numpy as np
 import pytest
@@ -26,9 +27,10 @@ def _release_buffers():
 
 
 def plain(cache, q, starts, pos, tables, window=0, keep=0):
-    """float64: results, A [T][H][Dv]; R, S, n [T][H][1]"""
+    """float64: results, A [T][H][Dv]; R, S, Q, n [T][H][1]"""
     T, H, _ = q.shape
-    out, A, R, S, n = np.zeros((T, H, cache.Dv)), np.zeros((T, H, cache.Dv)), np.zeros((T, H, 1)), np.zeros((T, H, 1)), np.zeros((T, H, 1))
+    out, A = np.zeros((T, H, cache.Dv)), np.zeros((T, H, cache.Dv))
+    R, S, Q, n = np.zeros((4, T, H, 1))
     for s in range(len(pos)):
         t0, new, p0 = int(starts[s]), int(starts[s + 1] - starts[s]), int(pos[s])
         k, v = cache.numbers(tables[s], p0 + new)
@@ -45,14 +47,15 @@ def plain(cache, q, starts, pos, tables, window=0, keep=0):
                 w /= w.sum()
                 out[t0 + i, h], A[t0 + i, h] = w @ v[seen, g], w @ np.abs(v[seen, g])
                 R[t0 + i, h], S[t0 + i, h], n[t0 + i, h] = P.TOP[cache.code] * (w @ step[seen, g]), (np.abs(k[seen, g]) @ np.abs(x)).max(), seen.sum()
-    return out, A, R, S, n
+                Q[t0 + i, h] = np.abs(k[seen, g]).sum(1).max() * np.abs(x).max()
+    return out, A, R, S, Q, n
 
 
 def check(dt, got, form, D):
-    out, A, R, S, n = form
+    out, A, R, S, Q, n = form
     tol = ((2 * (D + 8) * S + n + 64) * U + 2.0 ** -21) * A + n * 2.0 ** -32 * R
     if dt == BF16:
-        tol = tol + (2 * S + 1) * 2.0 ** -11 * A
+        tol = tol + (2.0 ** -19 * Q + 2.0 ** -11) * A
         tol = tol + 2.0 ** -8 * (np.abs(out) + tol)
     bad = ~(np.abs(got - out) <= tol)
     assert not bad.any(), f"{bad.sum()} of {bad.size} out of bounds, first {np.argwhere(bad)[0]}: {got[bad][0]} for {out[bad][0]}, {(np.abs(got - out) / tol)[bad].max()} times the bound"
@@ -153,3 +156,27 @@ def test_scales_far_apart(gpu, dt, code, T, H, D, kind):
             if kind == "edges" and j % 5 == 0:
                 cache.v[tables[0, j // 2], :, 16 * (j % 2):16 * (j % 2) + 16] = 0
     both(gpu, dt, cache, q, starts, [400], tables, T)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("T,H", [(1, 4), (3, 4), (40, 4)])
+@pytest.mark.parametrize("score", [5, 40, 80])
+def test_equal_scores_along_different_numbers(gpu, dt, code, T, H, score):
+    """two halves of the keys with the same large score, one by numbers of the query that 11 bits cut, the other by numbers that they hold, and values of either sign: what is cut off a
+    query a score multiplies"""
+    D = 64
+    r, cache, starts, tables, q = made(code, T, H, D, 64, 6)
+    top = P.TOP[code]
+    cache.k[...], cache.scales[:, :, 0] = 0, 1.0
+    cache.v[...], cache.scales[:, :, 1] = P.encode(code, np.full(1, top, np.float32))[0], 1 / top
+    one = P.encode(code, np.full(1, 1, np.float32))[0]
+    for j in range(64 + T):
+        page, row = tables[0, j // 32], j % 32
+        cache.k[page, 0, row, :32 if j % 2 else 0] = one
+        cache.k[page, 0, row, 32:(32 if j % 2 else 64)] = one
+        if j % 2:
+            cache.v[page, 0, row] = P.encode(code, np.full(1, -top / 2, np.float32))[0]
+    q[...] = score / 32
+    q[..., :32] *= np.float32(1 + 2.0 ** -11 * 0.99)
+    both(gpu, dt, cache, q, starts, [64], tables, T)
