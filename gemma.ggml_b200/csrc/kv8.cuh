@@ -10,6 +10,8 @@
 #include <cuda_fp8.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "dense.cuh"
 #include "tc.cuh"
 
@@ -66,7 +68,7 @@ struct attn_args {
     const float *sink, *gate;
     int64_t ldg, record;
     void *out;
-    int groups;     // items of a sequence and key head, at most
+    int entries, groups; // places for the items of a key head (list_items); as many for every sequence, or 0
     int64_t rows_above, rows_up_to; // sequences of more rows (tokens x query heads of a key head) than the one, up to the other, are this kernel's
     float *part;    // pieces' sums [CTA][2][rows][Dv], or null: an item a CTA
     float2 *part_ml; // their maxima and denominators [CTA][2][rows]
@@ -136,10 +138,11 @@ struct item {
 template <int R, int TILE> __device__ __forceinline__ item item_of(const attn_args &a, int s, int rg) {
     item x;
     const int hpg = a.H / a.G;
-    x.s = s, x.rg = rg, x.t0 = a.starts[s], x.p0 = a.pos0[s], x.row0 = rg * R;
+    x.s = s, x.rg = rg, x.n = 0;
+    if (s >= a.n_seq) return x; // behind the last place
+    x.t0 = a.starts[s], x.p0 = a.pos0[s], x.row0 = rg * R;
     const int64_t all = (a.starts[s + 1] - x.t0) * hpg;
     x.rows = (int)min((int64_t)R, all - x.row0);
-    x.n = 0;
     if (x.rows <= 0 || all <= a.rows_above || all > a.rows_up_to) return x;
     x.i0 = x.p0 + x.row0 / hpg, x.i1 = x.p0 + (x.row0 + x.rows - 1) / hpg;
     x.lo = a.window > 0 ? (int)max((int64_t)0, x.i0 - a.window + 1) : 0;
@@ -162,6 +165,37 @@ struct piece {
     int entry, head, tile, n;
     unsigned u; // the head's first unit
 };
+// The places of a head's items, R rows each.  Either every sequence has as many as max_new tokens take, or sequence s those from starts[s] * (H / G) / R + s on, at least as many as
+// its rows fill: whichever are fewer, since every CTA goes through all of them, and limits count them (512 sequences of which one brings 8,192 tokens, eight query heads a key head: 262,144 places
+// of 128 rows, or 1,055)
+template <int R> __device__ __forceinline__ int first_place(const attn_args &a, int s) { return (int)((int64_t)a.starts[s] * (a.H / a.G) / R) + s; }
+template <int R, int TILE> __device__ __forceinline__ void to_entry(const attn_args &a, piece &x, int entry) {
+    int s, rg;
+    if (a.groups > 0) {
+        s = entry / a.groups, rg = entry - s * a.groups;
+    } else {
+        int n = a.n_seq + 1; // the last place that is not behind
+        for (s = 0; n > 1;) {
+            const int half = n / 2;
+            if (first_place<R>(a, s + half) <= entry) s += half, n -= half;
+            else n = half;
+        }
+        rg = entry - first_place<R>(a, s);
+    }
+    x.entry = entry, x.it = item_of<R, TILE>(a, s, rg);
+}
+template <int R, int TILE> __device__ __forceinline__ void next_entry(const attn_args &a, piece &x) {
+    int s = x.it.s, rg = x.it.rg + 1;
+    x.entry++;
+    if (s < a.n_seq && (a.groups > 0 ? rg == a.groups : x.entry == first_place<R>(a, s + 1))) s++, rg = 0;
+    x.it = item_of<R, TILE>(a, s, rg);
+}
+// places of R rows for calls of up to T tokens, max_new a sequence
+inline int64_t list_items(attn_args &a, int64_t T, int64_t max_new, int R) {
+    const int64_t hpg = a.H / a.G, groups = (max_new * hpg + R - 1) / R, even = a.n_seq * groups, own = T * hpg / R + a.n_seq;
+    a.groups = even <= own ? (int)groups : 0; // (no more than own, which is below 2^31 where it is used)
+    return std::min(even, own);
+}
 // the first piece from unit `at` on, which lies in the head that begins at x.u; n 0: none ahead of `end`
 template <int R, int TILE, int kBegin> __device__ __forceinline__ void piece_from(const attn_args &a, piece &x, unsigned at, unsigned end) {
     for (;;) {
@@ -171,10 +205,8 @@ template <int R, int TILE, int kBegin> __device__ __forceinline__ void piece_fro
         if (at >= end) return;
         if (++x.head == a.G) {
             x.head = 0;
-            do {
-                x.entry++;
-                x.it = item_of<R, TILE>(a, x.entry / a.groups, x.entry % a.groups);
-            } while (x.it.n == 0);
+            do next_entry<R, TILE>(a, x);
+            while (x.it.n == 0);
         }
     }
 }

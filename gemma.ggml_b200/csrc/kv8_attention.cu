@@ -175,13 +175,14 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
 
     // ---- what this CTA has been dealt
     if (a.part) {
-        const int entries = a.n_seq * a.groups, each = (entries + Z::threads - 1) / Z::threads, e0 = min(entries, tid * each), e1 = min(entries, e0 + each);
+        const int each = (a.entries + Z::threads - 1) / Z::threads, e0 = min(a.entries, tid * each), e1 = min(a.entries, e0 + each);
         unsigned mine = 0, U = 0, base = 0;
         piece x;
-        for (x.entry = e0; x.entry < e1; x.entry++) {
-            x.it = item_of<R, Z::tile>(a, x.entry / a.groups, x.entry % a.groups);
-            if (x.it.n) mine += (x.it.n + kBegin) * a.G;
-        }
+        if (e0 < e1)
+            for (to_entry<R, Z::tile>(a, x, e0);; next_entry<R, Z::tile>(a, x)) {
+                if (x.it.n) mine += (x.it.n + kBegin) * a.G;
+                if (x.entry + 1 == e1) break;
+            }
         unsigned run = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -201,21 +202,19 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
         base += run - mine;
         if (u < end && u >= base && u < base + mine) {
             if (each > 1)
-                for (x.entry = e0;; x.entry++) {
-                    x.it = item_of<R, Z::tile>(a, x.entry / a.groups, x.entry % a.groups);
+                for (to_entry<R, Z::tile>(a, x, e0);; next_entry<R, Z::tile>(a, x)) {
                     const unsigned n = x.it.n ? (x.it.n + kBegin) * a.G : 0;
                     if (u < base + n) break;
                     base += n;
                 }
-            else x.entry = e0;
             x.head = (int)((u - base) / (unsigned)(x.it.n + kBegin)), x.u = base + x.head * (x.it.n + kBegin);
             piece_from<R, Z::tile, kBegin>(a, x, u, end);
             s_piece[0] = x, s_end = end, s_all = U;
         }
     } else if (tid == 0) {
         piece x;
-        x.entry = blockIdx.x / a.G, x.head = blockIdx.x - x.entry * a.G, x.tile = 0, x.u = 0;
-        x.it = item_of<R, Z::tile>(a, x.entry / a.groups, x.entry % a.groups);
+        to_entry<R, Z::tile>(a, x, blockIdx.x / a.G);
+        x.head = blockIdx.x - x.entry * a.G, x.tile = 0, x.u = 0;
         x.n = x.it.n;
         s_piece[0] = x, s_end = 0, s_all = 0;
     }
@@ -681,17 +680,17 @@ template <int R, typename E> __global__ void __launch_bounds__(256) kv8_join_ker
     }
 }
 
-template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64_t max_new) {
+template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64_t T, int64_t max_new) {
     using Z = step_sizes<CODE, P, NT, PARTS>;
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;
-    const int64_t groups = (max_new * (a.H / a.G) + Z::R - 1) / Z::R;
-    GGB_CHECK_ARG(max_new * (a.H / a.G) < (1ll << 30) && a.n_seq * groups * a.G < (1ll << 31), "kv8_attn: too many sequences, tokens and heads for a launch");
-    GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.positions + a.keep) / Z::tile + 4) < (1ll << 31), "kv8_attn: too many positions for a launch"); // the units of a deal, at most
-    a.groups = (int)groups;
+    const int64_t places = list_items(a, T, max_new, Z::R);
+    GGB_CHECK_ARG(max_new * (a.H / a.G) < (1ll << 30) && places * a.G < (1ll << 31), "kv8_attn: too many sequences, tokens and heads for a launch");
+    GGB_CHECK_ARG(places * a.G * ((a.positions + a.keep) / Z::tile + 4) < (1ll << 31), "kv8_attn: too many positions for a launch"); // the units of a deal, at most
+    a.entries = (int)places;
     auto k = kv8_step_kernel<CODE, P, NT, PARTS>;
     int rc = ggb_allow_smem(k, Z::smem);
     if (rc) return rc;
-    const unsigned ctas = a.part ? (unsigned)std::min(kMaxCtas, ggb_sm_count() * Z::min_ctas) : (unsigned)(a.n_seq * a.groups * a.G);
+    const unsigned ctas = a.part ? (unsigned)std::min(kMaxCtas, ggb_sm_count() * Z::min_ctas) : (unsigned)(a.entries * a.G);
     line_maps maps;
     rc = make_line_maps(a, maps);
     if (rc) return rc;
@@ -704,12 +703,12 @@ template <int CODE, int P, int NT, int PARTS> int step_launch(attn_args a, int64
     return GGB_OK;
 }
 // rows of an item: as many as a sequence and key head has, up to 32 (16 with the largest heads, whose sums fill the registers)
-template <int CODE, int PARTS> int step_rows(const attn_args &a, int64_t max_new) {
+template <int CODE, int PARTS> int step_rows(const attn_args &a, int64_t T, int64_t max_new) {
     const int64_t rows = max_new * (a.H / a.G);
     const int size = std::max(a.D, a.Dv);
-    if (size <= 64) return rows <= 8 ? step_launch<CODE, 64, 1, PARTS>(a, max_new) : rows <= 16 ? step_launch<CODE, 64, 2, PARTS>(a, max_new) : step_launch<CODE, 64, 4, PARTS>(a, max_new);
-    if (size <= 128) return rows <= 8 ? step_launch<CODE, 128, 1, PARTS>(a, max_new) : rows <= 16 ? step_launch<CODE, 128, 2, PARTS>(a, max_new) : step_launch<CODE, 128, 4, PARTS>(a, max_new);
-    return rows <= 8 ? step_launch<CODE, 256, 1, PARTS>(a, max_new) : step_launch<CODE, 256, 2, PARTS>(a, max_new);
+    if (size <= 64) return rows <= 8 ? step_launch<CODE, 64, 1, PARTS>(a, T, max_new) : rows <= 16 ? step_launch<CODE, 64, 2, PARTS>(a, T, max_new) : step_launch<CODE, 64, 4, PARTS>(a, T, max_new);
+    if (size <= 128) return rows <= 8 ? step_launch<CODE, 128, 1, PARTS>(a, T, max_new) : rows <= 16 ? step_launch<CODE, 128, 2, PARTS>(a, T, max_new) : step_launch<CODE, 128, 4, PARTS>(a, T, max_new);
+    return rows <= 8 ? step_launch<CODE, 256, 1, PARTS>(a, T, max_new) : step_launch<CODE, 256, 2, PARTS>(a, T, max_new);
 }
 
 // sequences of many rows by the tiles' kernel, the others by the steps', which begin and end sooner.  16 sequences at 2,000 positions (bf16, 16 heads over 4 of 128), steps
@@ -721,7 +720,7 @@ template <int CODE, int PARTS> int attend(attn_args a, int64_t T, int64_t max_ne
     const bool tiles = max_new * hpg > kFew && tile_fits(a.D, a.Dv, a.H, a.G), steps = !tiles || (a.n_seq > 1 && hpg <= kFew);
     if (steps) {
         a.rows_above = 0, a.rows_up_to = tiles ? kFew : INT64_MAX;
-        const int rc = step_rows<CODE, PARTS>(a, tiles ? kFew / hpg : max_new);
+        const int rc = step_rows<CODE, PARTS>(a, T, tiles ? kFew / hpg : max_new);
         if (rc) return rc;
     }
     if (tiles) {
@@ -762,7 +761,7 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
     const int64_t positions = std::min<int64_t>(table_ld, (1ll << 31) / block_size) * block_size; // (they are 32-bit numbers)
     float *part = (float *)scratch;
     const attn_args a{q, (const uint8_t *)cache, tables, table_ld, block_size, n_seq, starts, pos0, H, G, D, Dv, window, window > 0 ? std::min<int64_t>(keep_first, positions) : 0, softcap, sink, gate, ldg,
-                      kv8_record(D, Dv, block_size), out, 0, 0, 0, part, (float2 *)(part ? part + (size_t)kMaxCtas * 2 * kMaxRows * Dv : nullptr),
+                      kv8_record(D, Dv, block_size), out, 0, 0, 0, 0, part, (float2 *)(part ? part + (size_t)kMaxCtas * 2 * kMaxRows * Dv : nullptr),
                       (int4 *)(part ? part + (size_t)kMaxCtas * 2 * kMaxRows * (Dv + 2) : nullptr), (uintptr_t)q % 16 == 0,
                       (uintptr_t)out % 16 == 0, (uintptr_t)gate % 16 == 0 && ldg % 4 == 0, positions, ggb_wait_error_flag()};
     if (dt == GGB_TYPE_BF16) return code == GGB_KV8_INT8 ? attend<GGB_KV8_INT8, 1>(a, T, max_new) : attend<GGB_KV8_E4M3, 1>(a, T, max_new);

@@ -129,10 +129,8 @@ __device__ __forceinline__ void tile_piece_from(const attn_args &a, piece &x, un
         if (x.u >= end) return;
         if (++x.head == a.G) {
             x.head = 0;
-            do {
-                x.entry++;
-                x.it = item_of<kTileRows, kTileKeys>(a, x.entry / a.groups, x.entry % a.groups);
-            } while (x.it.n == 0);
+            do next_entry<kTileRows, kTileKeys>(a, x);
+            while (x.it.n == 0);
         }
     }
     x.tile = 0, x.n = x.it.n;
@@ -173,13 +171,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
 
     // ---- what this CTA has been dealt
     {
-        const int entries = a.n_seq * a.groups, each = (entries + kTileThreads - 1) / kTileThreads, e0 = min(entries, tid * each), e1 = min(entries, e0 + each);
+        const int each = (a.entries + kTileThreads - 1) / kTileThreads, e0 = min(a.entries, tid * each), e1 = min(a.entries, e0 + each);
         unsigned mine = 0, U = 0, front = 0;
         piece x;
-        for (x.entry = e0; x.entry < e1; x.entry++) {
-            x.it = item_of<kTileRows, kTileKeys>(a, x.entry / a.groups, x.entry % a.groups);
-            if (x.it.n) mine += (x.it.n + kTileBegin) * a.G;
-        }
+        if (e0 < e1)
+            for (to_entry<kTileRows, kTileKeys>(a, x, e0);; next_entry<kTileRows, kTileKeys>(a, x)) {
+                if (x.it.n) mine += (x.it.n + kTileBegin) * a.G;
+                if (x.entry + 1 == e1) break;
+            }
         unsigned run = mine;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -203,8 +202,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
         const unsigned u = d.first(blockIdx.x), end = d.first(blockIdx.x + 1);
         front += run - mine;
         if (u < end && u >= front && u < front + mine) {
-            for (x.entry = e0;; x.entry++) {
-                x.it = item_of<kTileRows, kTileKeys>(a, x.entry / a.groups, x.entry % a.groups);
+            for (each > 1 ? to_entry<kTileRows, kTileKeys>(a, x, e0) : void();; next_entry<kTileRows, kTileKeys>(a, x)) {
                 const unsigned n = x.it.n ? (x.it.n + kTileBegin) * a.G : 0;
                 if (u < front + n) break;
                 front += n;
@@ -635,9 +633,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tile_kernel(const __grid_
 // *joins: CTAs whose pieces are to be joined.  Few items are cut, an even share for kTileCtas; of many, whole ones make shares that are even enough, for every SM
 template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t max_new, unsigned *joins) {
     const int hpg = a.H / a.G;
-    const int64_t groups = (max_new * hpg + kTileRows - 1) / kTileRows, items = (T * hpg + kTileRows - 1) / kTileRows * a.G;
-    GGB_CHECK_ARG(a.n_seq * groups * a.G * ((a.positions + a.keep) / kTileKeys + kTileBegin + 2) < (1ll << 31), "kv8_attn: too many sequences, tokens, heads and positions for a launch");
-    a.groups = (int)groups;
+    const int64_t places = list_items(a, T, max_new, kTileRows), items = (T * hpg + kTileRows - 1) / kTileRows * a.G;
+    GGB_CHECK_ARG(places * a.G * ((a.positions + a.keep) / kTileKeys + kTileBegin + 2) < (1ll << 31), "kv8_attn: too many sequences, tokens, heads and positions for a launch");
+    a.entries = (int)places;
     // (bf16 results, 16 heads over 4 of 128, 4,096 tokens, 3.5 items an SM: whole 202 us, cut 223; 2,500 tokens in fp32, where what a chain leaves goes to memory and back, 187 and
     // 164, 4,096 tokens 397 and 360)
     if (items >= (PARTS == 1 ? 3 : 8) * ggb_sm_count()) a.part = nullptr;

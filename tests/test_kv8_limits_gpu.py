@@ -194,3 +194,40 @@ def test_portions_whose_last_rows_end_inside_a_warp(gpu, dt, new, Dv):
     want, reach = P.attention(cache, q, starts, pos, np.maximum(tables, 0), 33, 2, gate=gate)
     for scratch in (True, False):
         check_attention(dt, run_attention(gpu, dt, cache, q, n, starts, pos, tables, max(new), 33, 2, gate=gate, scratch=scratch), want, reach, 64, 240)
+
+
+@pytest.mark.parametrize("dt,D", [(F32, 64), (BF16, 64), (BF16, 256)])
+def test_a_ragged_batch_with_room_for_long_sequences(gpu, dt, D):
+    """512 sequences whose buffers hold 4,096 tokens, any of them in one sequence, and whose page tables hold a million positions: every sequence with as many items as the longest could have would be
+    more than a launch counts, the items that 4,096 tokens can make are not"""
+    r = np.random.default_rng(19)
+    new = [int(x) for x in r.integers(0, 3, 512)]
+    new[100], new[511], new[200:210] = 50, 21, [0] * 10
+    pos = [int(x) for x in r.integers(0, 40, 512)]
+    starts, few, pages = batch(r, new, pos, 128)
+    cache = P.Cache(P.E4M3, 2, D, D, 128, pages).filled(r)
+    poison(cache, few, pos, new, True)
+    tables = np.full((512, 8192), -1, np.int32)
+    tables[:, :few.shape[1]] = few
+    q = f32(r.standard_normal((sum(new), 16, D)) * 0.2)
+    want, reach = P.attention(cache, q, starts, pos, np.maximum(few, 0))
+    for scratch in (True, False):
+        got = run_attention(gpu, dt, cache, q, 4096, starts, pos, tables, 4096, scratch=scratch)
+        check_attention(dt, got, want, reach, D, 100)
+        if scratch:
+            assert np.array_equal(got, run_attention(gpu, dt, cache, q, 4096, starts, pos, few, 50))  # the same items in the same order, however they are listed
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_one_portion_among_many_steps(gpu, dt):
+    """places by tokens: sequences without any, with one and with many rows behind one another"""
+    r = np.random.default_rng(20)
+    new = [0, 0, 130, 1, 0, 1, 1, 0] + [1] * 90 + [0, 0]
+    pos = [int(x) for x in r.integers(0, 300, len(new))]
+    starts, tables, pages = batch(r, new, pos, 16)
+    cache = P.Cache(P.INT8, 1, 64, 64, 16, pages).filled(r)
+    poison(cache, tables, pos, new, True)
+    q = f32(r.standard_normal((sum(new), 3, 64)) * 0.2)
+    want, reach = P.attention(cache, q, starts, pos, np.maximum(tables, 0), 100, 5)
+    for scratch in (True, False):
+        check_attention(dt, run_attention(gpu, dt, cache, q, len(q) + 5, starts, pos, tables, 130, 100, 5, scratch=scratch), want, reach, 64, 300)
