@@ -403,7 +403,7 @@ size_t ggb_draft_verify_scratch_bytes(int64_t R, int n_seq) {
 int ggb_op_draft_verify(const float *target, int64_t ld_target, const float *draft, int64_t ld_draft, int64_t V, int64_t R, int n_seq, const int32_t *starts,
                         const int32_t *drafted, const float *u, float temperature, int32_t *tokens, int32_t *n_accepted, void *scratch, size_t scratch_bytes) {
     GGB_REQUIRE_INIT();
-    GGB_CHECK_ARG(target && starts && drafted && u && tokens && n_accepted && scratch, "draft_verify: a pointer is null");
+    GGB_CHECK_ARG(target && starts && drafted && (u || temperature == 0.f) && tokens && n_accepted && scratch, "draft_verify: a pointer is null");
     GGB_CHECK_ARG(V > 0 && V < (1ll << 31) - (1 << 20) && R > 0 && R <= 65535 && n_seq > 0 && n_seq <= 65535, "draft_verify: %lld rows of %lld numbers, %d sequences", (long long)R,
                   (long long)V, n_seq);
     GGB_CHECK_ARG(ld_target >= V && (!draft || ld_draft >= V), "draft_verify: rows of %lld numbers overlap", (long long)V);

@@ -532,7 +532,7 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
  * temperature), q = soft-max(draft / temperature) (draft NULL: 1 at the drafted token).  The token d of a row stands where u[row] q(d) < p(d); n_accepted[s] stand before
  * the first that does not.  Behind them one is drawn: of the row where a draft fell from max(p - q, 0) over its sum (should that be nothing: from p), of the last
  * row where all stand from p: the first v where the running sum exceeds u[last row] times the whole.  temperature 0: a token stands where it is the first maximum, which
- * is also drawn (draft and u are not read).  tokens[starts[s] + j]: the tokens that stand, the drawn one, then -1.  Logits of -inf have probability 0; a row with NaN or
+ * is also drawn (draft and u are not read and may be NULL).  tokens[starts[s] + j]: the tokens that stand, the drawn one, then -1.  Logits of -inf have probability 0; a row with NaN or
  * +inf (temperature 0: with NaN), or with nothing above -inf, has no distribution: no token stands by it and -1 is drawn.  A drafted token outside of [0, V) falls.
  * scratch: ggb_draft_verify_scratch_bytes, on a 16-byte boundary. */
 size_t ggb_draft_verify_scratch_bytes(int64_t R, int n_seq);

@@ -191,3 +191,17 @@ def test_a_long_row_where_nothing_is_left_of_the_difference(gpu):
     target = np.zeros((4, V), np.float32)
     got, acc = run(gpu, target, target, [0, 2, 4], [5, 0, 5, 0], np.array([1.0, 0.9, 1.0, 0.125], np.float32), 1.0)
     assert list(acc) == [0, 0] and list(got) == [int(np.floor(np.float64(np.float32(0.9)) * V)), -1, V // 8, -1]
+
+
+def test_greedy_without_random_numbers(gpu):
+    """at temperature 0 neither the draft's logits nor random numbers are read: there need not be any"""
+    lib, r = gpu.cuda_lib(), np.random.default_rng(40)
+    target, _, starts, _ = inputs(r, [4, 1, 3], 500)
+    drafted = i32(target.argmax(1))
+    drafted[5] += 1
+    nbytes = int(lib.ggb_draft_verify_scratch_bytes(8, 3))
+    tokens, accepted, scratch = dev(gpu, np.full(8, -2, np.int32)), dev(gpu, np.full(3, -2, np.int32)), zeros(gpu, nbytes)
+    a = [dev(gpu, x) for x in (target, starts, drafted)]
+    gpu.check(lib.ggb_op_draft_verify(a[0].ptr, 500, None, 0, 500, 8, 3, a[1].ptr, a[2].ptr, None, 0.0, tokens.ptr, accepted.ptr, scratch.ptr, nbytes), "draft_verify")
+    want, acc, _ = P.verify(target, None, starts, drafted, np.zeros(8, np.float32), 0.0)
+    assert np.array_equal(tokens.download(np.int32), want) and np.array_equal(accepted.download(np.int32), acc) and list(acc) == [3, 0, 0]
