@@ -11,9 +11,12 @@
 //   pick    a CTA a piece of the row that is drawn from: joins the rows' pieces, decides what stands, sums its piece of the weights; the CTA that is done last finds
 //           the token: the piece by the pieces' sums in order, the part of it by its warps', then the place in that
 //
-// Exponentials in fp32 and sums of four of them; beyond that, sums, and the probabilities that judge a draft, in 64 bits.  A weight p - q is a 32-bit difference of
-// 32-bit products: as far off as its exponentials are, and nothing where p and q are the same numbers.  So a decision is another one than in 64 bits throughout only
-// where the numbers compared are within about 1e-7 of one another.  Sums are added in an order that the sizes alone set.
+// Exponentials in fp32 and sums of four of them; beyond that, sums, and the probabilities that judge a draft, in 64 bits.  An exponential is off by 4 steps of 2^-24 of itself
+// (the unit) and by three more (difference, constant, product) times its argument, which is below 20 where a weight counts: p and q are off by less than 4e-6 of
+// themselves.  So a draft is judged otherwise than in 64 bits throughout only where u q and p are within twice that of one another.  A weight p - q is a 32-bit difference of 32-bit products,
+// nothing where p and q are the same numbers; running sums of them are off by up to 8e-6, and the whole is, so the token that is drawn is one whose part of the
+// running sum lies within 1.6e-5, over the sum of what is left, of u.  (Of a draft that is nearly the target 1e-5 may be left: then that says little, once in 1e5 rows.)  Sums are added in an
+// order that the sizes alone set.
 //
 // What bounds it: for large batches the instructions of the exponentials beside the bytes of the logits, read once (16 sequences of up to five drafts, 256,000 numbers: 39.8 us,
 // some 25 of them in the first kernel, where the bytes take 16.3), and what the second does one thing after the other; for one sequence (11.3 us) and the greedy form (24

@@ -534,6 +534,7 @@ int ggb_op_kv8_attn(int dt, int code, const float *q, const void *cache, const i
  * row where all stand from p: the first v where the running sum exceeds u[last row] times the whole.  temperature 0: a token stands where it is the first maximum, which
  * is also drawn (draft and u are not read and may be NULL).  tokens[starts[s] + j]: the tokens that stand, the drawn one, then -1.  Logits of -inf have probability 0; a row with NaN or
  * +inf (temperature 0: with NaN), or with nothing above -inf, has no distribution: no token stands by it and -1 is drawn.  A drafted token outside of [0, V) falls.
+ * p and q are 32-bit numbers, off by up to 4e-6 of themselves: so are the borders that u is compared with, those of max(p - q, 0) by 1.6e-5 over its sum.
  * scratch: ggb_draft_verify_scratch_bytes, on a 16-byte boundary. */
 size_t ggb_draft_verify_scratch_bytes(int64_t R, int n_seq);
 int ggb_op_draft_verify(const float *target, int64_t ld_target, const float *draft, int64_t ld_draft, int64_t V, int64_t R, int n_seq, const int32_t *starts,

@@ -205,3 +205,28 @@ def test_greedy_without_random_numbers(gpu):
     gpu.check(lib.ggb_op_draft_verify(a[0].ptr, 500, None, 0, 500, 8, 3, a[1].ptr, a[2].ptr, None, 0.0, tokens.ptr, accepted.ptr, scratch.ptr, nbytes), "draft_verify")
     want, acc, _ = P.verify(target, None, starts, drafted, np.zeros(8, np.float32), 0.0)
     assert np.array_equal(tokens.download(np.int32), want) and np.array_equal(accepted.download(np.int32), acc) and list(acc) == [3, 0, 0]
+
+
+@pytest.mark.parametrize("apart", [0.3, 3e-3, 3e-5])
+@pytest.mark.parametrize("V", [300, 50000])
+def test_drawn_from_what_little_is_left(gpu, apart, V):
+    """drafts that are nearly the target: p - q adds up to some 0.4 apart.  Where one falls, the token that is drawn has a part of the running sum of max(p - q, 0) that u lies in, within the
+    bound over that sum: p and q off by NEAR of themselves, so the running sum by 2 NEAR, and u times the whole by that again"""
+    r = np.random.default_rng(41)
+    n = 60
+    target = f32(r.standard_normal((2 * n, V)) * 2.0)
+    draft = f32(target + apart * r.standard_normal((2 * n, V)))
+    p, q = (np.exp(x.astype(np.float64) - x.max(1, keepdims=True)) for x in (target, draft))
+    p, q = p / p.sum(1, keepdims=True), q / q.sum(1, keepdims=True)
+    drafted = i32((q - p).argmax(1))  # q above p: u = 1 lets it fall
+    u = f32(np.stack([np.ones(n), (np.arange(n) + 0.5) / n], 1).ravel())
+    starts = i32(2 * np.arange(n + 1))
+    got, accepted = run(gpu, target, draft, starts, drafted, u, 1.0)
+    sure = (q > p * (1 + 4 * NEAR))[2 * np.arange(n), drafted[::2]]
+    assert sure.sum() > n // 2 and (accepted[sure] == 0).all()
+    assert P.agrees(got, accepted, target, draft, starts, drafted, u, 1.0, NEAR)
+    for s in np.nonzero(accepted == 0)[0]:
+        run_ = np.cumsum(np.maximum(p[2 * s] - q[2 * s], 0))
+        v, left, slack = int(got[2 * s]), run_[-1], 4 * NEAR / run_[-1]
+        assert run_[v] / left > u[2 * s + 1] - slack and (v == 0 or run_[v - 1] / left <= u[2 * s + 1] + slack)
+        assert p[2 * s, v] - q[2 * s, v] > -NEAR * (p[2 * s, v] + q[2 * s, v])  # of the tokens that are left, but for what p and q are off
