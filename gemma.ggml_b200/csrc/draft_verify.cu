@@ -18,8 +18,9 @@
 // running sum lies within 1.6e-5, over the sum of what is left, of u.  (Of a draft that is nearly the target 1e-5 may be left: then that says little, once in 1e5 rows.)  Sums are added in an
 // order that the sizes alone set.
 //
-// What bounds it: for large batches the instructions of the exponentials beside the bytes of the logits, read once (16 sequences of up to five drafts, 256,000 numbers: 39.8 us,
-// some 25 of them in the first kernel, where the bytes take 16.3), and what the second does one thing after the other; for one sequence (11.3 us) and the greedy form (24
+// What bounds it: for large batches (16 sequences of up to five drafts, 256,000 numbers: 39.9 us, some 25 of them in the first kernel, where the bytes of the logits, read once, take
+// 16.3) neither bytes nor instructions alone (DRAM 57 % and issue 57 % of their peaks, 15 instructions a number): a CTA has one block of numbers, so nothing is on its way while it
+// finds the block's maximum and adds up; and what the second kernel does one thing after the other.  For one sequence (11.3 us) and the greedy form (24
 // sequences, 49,999 numbers: 7.9 us, the bytes 3.3) the two launches and that chain.
 #include <algorithm>
 
@@ -74,8 +75,8 @@ __device__ __forceinline__ float4 load4(const float *x, int i, int n, bool vec) 
     for (int e = 0; e < 4; e++) y[e] = i + e < n ? x[i + e] : -INFINITY;
     return make_float4(y[0], y[1], y[2], y[3]);
 }
-// exp((x - m) / temperature) as a power of two, c = log2(e) / temperature: the unit's 2^-22 and the argument's roundings of 2^-24 of itself.  Above expf that saves its
-// steps for large arguments, five of the ten instructions a number; below 2^-126 it is zero.
+// exp((x - m) / temperature) as a power of two, c = log2(e) / temperature: the unit's 2^-22 and the argument's roundings of 2^-24 of itself.  It takes none of
+// expf's steps for large arguments; below 2^-126 it is zero.
 __device__ __forceinline__ float power(float x, float m, float c) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x - m) * c));

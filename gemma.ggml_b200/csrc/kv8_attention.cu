@@ -21,8 +21,8 @@
 // ragged batches and single long sequences fill the chip alike.  A CTA that has only a piece of an item leaves it in the workspace (the first or the last
 // of what it was dealt: two places), and kv8_join_kernel adds an item's pieces up in order.
 //
-// What bounds it: from some ten megabytes of codes on the bytes (32 sequences of 8,000 positions, 32 heads over 8 of 128: 62.7 us, 79 % of what a copy moves; of 32,000
-// 207 us, 95 %).  Below that what a launch has to do one after the other: look up what was dealt (1.3 us), queries and the first codes (2.5), the warps' sums (1.1), the join (3.5).
+// What bounds it: from some ten megabytes of codes on the bytes (32 sequences of 8,000 positions, 32 heads over 8 of 128: 63.3 us, 78 % of what a copy moves; of 32,000
+// 203 us, 97 %).  Below that what a launch has to do one after the other: look up what was dealt (1.3 us), queries and the first codes (2.5), the warps' sums (1.1), the join (3.5).
 #include <algorithm>
 #include <type_traits>
 
@@ -68,7 +68,7 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
 template <int CODE, int P, int NT, int PARTS> struct step_sizes {
     static constexpr int R = 8 * NT, KS = P / 16; // blocks of 16 value coordinates
     // groups of 16 keys that a warp takes at once: two where the sums leave registers for them, which also gives the warp independent work (32 sequences of 8,000 positions, 128
-    // numbers: 62.9 us, one 66.3; with two more drafted tokens each 94 and 107); with heads of 256, whose sums fill the registers, one (41 us, two 44).  Two CTAs of six warps
+    // numbers: 63.6 us, one 66.8; with two more drafted tokens each 97 and 108); with heads of 256, whose sums fill the registers, one (16 over 2: 42.7 us, two 46.1).  Two CTAs of six warps
     // an SM, or one of eight
     static constexpr int min_ctas = P * NT <= 128 ? 2 : 1, W = min_ctas == 2 ? 6 : 8, U = P < 256 && P * NT <= 256 ? 2 : 1, threads = 32 * W, tile = 16 * W * U;
     // queries: int8 digits for steps of 32 numbers, or fp16 parts for steps of 16
@@ -711,8 +711,9 @@ template <int CODE, int PARTS> int step_rows(const attn_args &a, int64_t T, int6
     return rows <= 8 ? step_launch<CODE, 256, 1, PARTS>(a, T, max_new) : step_launch<CODE, 256, 2, PARTS>(a, T, max_new);
 }
 
-// sequences of many rows by the tiles' kernel, the others by the steps', which begin and end sooner.  16 sequences at 2,000 positions (bf16, 16 heads over 4 of 128), steps
-// against tiles: 64 rows 41 and 52 us, 96 rows 47 and 62, 128 rows 56 and 68; one sequence 17, 19, 19 and 22, 23, 25.  Beyond that tiles of 128 rows are not empty in part
+// sequences of many rows by the tiles' kernel, the others by the steps', which begin and end sooner.  One sequence at 2,000 positions (bf16, 16 heads over 4 of 128), steps against tiles: 64 rows
+// 16.9 and 21.4 us, 96 rows 18.9 and 22.5, 128 rows 18.8 and 23.7, 256 rows 26.7 and 24.4.  16 sequences of up to 256 rows: 87 by steps, 82 by both kernels, one behind the other, as a batch with shorter
+// sequences beside takes them; up to 132 rows 59 and 81.  (Were all rows of such a batch the tiles' kernel's: 41 us with 128 rows, where steps take 57, and 37 with 64, where they take 40.)
 constexpr int64_t kFew = 128;
 template <int CODE, int PARTS> int attend(attn_args a, int64_t T, int64_t max_new) {
     using E = typename std::conditional<PARTS == 1, __nv_bfloat16, float>::type;

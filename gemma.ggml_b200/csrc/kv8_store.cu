@@ -9,8 +9,8 @@
 // One launch: a CTA owns one (group, key head) that new tokens reach, a thread 16 numbers of a row; the CTAs behind those turn a token's queries each.  Multiply
 // and add round apart (as everywhere in this library), so codes are the same bits as those of the formulas in 32-bit arithmetic.
 //
-// What bounds it: single tokens the launch (one 2.5 us, 64 of different sequences 5.6 us); portions the bytes of the projections and of the turned queries (4,096
-// tokens, 32 heads over 8 of 128: 42.5 us, 4.6 TB/s, 71 % of what a copy moves; 55 us when a query's loads waited for its sequence, cosines and one another).
+// What bounds it: single tokens the launch (in replays of a captured graph, one 2.6 us, 64 of different sequences 5.6 us; call by call the host takes longer); portions the bytes of the projections and of the turned queries (4,096
+// tokens, 32 heads over 8 of 128: 42.9 us, 4.6 TB/s, 70 % of what a copy moves; 55 us when a query's loads waited for its sequence, cosines and one another).
 #include <algorithm>
 
 #include "kv8.cuh"

@@ -16,10 +16,10 @@
 // Work is dealt as in the steps' kernel: items (sequence, 128 rows, key head) of tiles in one row, an even share to every CTA, pieces of items joined behind; where there are
 // many items, whole ones.
 //
-// What bounds it: nothing is full.  A tile takes a group about 2 us and both together 1: weights some 1,600 cycles a tile and group, products (queries and keys from shared
-// memory, which the code warps write at the same time) some 1,300 where 650 would do.  Beside that an item begins in 6 us (what was dealt, queries, the first codes) and ends in
-// 4 to 8 (sums, gate, pieces).  1,024 tokens behind 1,024, window 1,024, 16 heads over 4 of 128, bf16, gate: 38 us (230 TFLOP/s; 128 us by the steps' kernel); 4,096 tokens
-// from position 0: 202 us (340 TFLOP/s).
+// What bounds it: nothing is full.  With one part of the queries a tile took a group about 2 us and both together 1: weights some 1,600 cycles a tile and group, products (queries and
+// keys from shared memory, which the code warps write at the same time) some 1,300 where 650 would do; the second part adds a third of a microsecond a tile, from shared memory or
+// from tensor memory.  Beside that an item begins in 6 us (what was dealt, queries, the first codes) and ends in 4 to 8 (sums, gate, pieces).  1,024 tokens behind 1,024, window 1,024,
+// 16 heads over 4 of 128, bf16, gate: 41.7 us (207 TFLOP/s; one part 38); 4,096 tokens from position 0: 254 us (270 TFLOP/s; one part 200), 8,192: 788 us (349 TFLOP/s).
 #pragma once
 
 #include "kv8.cuh"
@@ -636,8 +636,8 @@ template <int CODE, int PARTS> int tile_launch(attn_args a, int64_t T, int64_t m
     const int64_t places = list_items(a, T, max_new, kTileRows), items = (T * hpg + kTileRows - 1) / kTileRows * a.G;
     GGB_CHECK_ARG(places * a.G * ((a.positions + a.keep) / kTileKeys + kTileBegin + 2) < (1ll << 31), "kv8_attn: too many sequences, tokens, heads and positions for a launch");
     a.entries = (int)places;
-    // (bf16 results, 16 heads over 4 of 128, 4,096 tokens, 3.5 items an SM: whole 202 us, cut 223; 2,500 tokens in fp32, where what a chain leaves goes to memory and back, 187 and
-    // 164, 4,096 tokens 397 and 360)
+    // (bf16 results, 16 heads over 4 of 128, 4,096 tokens, 3.5 items an SM: with a window of 1,024 whole 133 us, cut 168; without one, from position 0 on, whole ones are uneven there, 254 and 236, and
+    // no longer with 10,240 tokens, 1,150 and 1,174.  In fp32, where what a chain leaves goes to memory and back, 2,560 tokens 177 and 153, 4,096 tokens 365 and 333, 16,384 4,087 and 4,279)
     if (items >= (PARTS == 1 ? 3 : 8) * ggb_sm_count()) a.part = nullptr;
     const size_t smem = std::max((size_t)tile_sizes(a.D, a.Dv).smem, kOneCtaSmem);
     auto kfn = kv8_tile_kernel<CODE, PARTS>;

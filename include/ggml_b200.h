@@ -517,8 +517,9 @@ int ggb_op_kv8_store(int code, const float *q, const float *k, const float *v, i
                      void *cache, float *q_out);
 /* Soft-max attention of q (fp32 [T][H * D], as ggb_op_kv8_store leaves it) over the cache, the batch's own new tokens in it: the query at position i sees j <= i, with
  * window > 0 only i - j < window or j < keep_first; softcap, sink (fp32 [H] or NULL) and gate (fp32 rows of stride ldg or NULL) as for ggb_op_masked_attn_gated; query
- * head h reads key head h / (H / G).  out (dt) [T][H * Dv].  max_new: no sequence brings more tokens than that (T at the most: what a call
- * costs goes by what sequences bring).  Taken is whatever has (T * H / G / 16 + n_seq) * G * ((positions of a table's row + keep_first) / 64 + 10) below 2^31.  A query that is not finite makes its own row NaN.
+ * head h reads key head h / (H / G).  out (dt) [T][H * Dv].  max_new: no sequence brings more tokens than that (T at the most: what a call costs goes by what the
+ * sequences bring).  Taken is whatever has (T * H / G / 16 + n_seq) * G * ((positions of a table's row + keep_first) / 64 + 10) below 2^31.  A query that is not finite makes
+ * its own row NaN.
  * What a position adds, its weight times its group's value scale, is taken with 11 bits for bf16 results and with 22 for fp32 ones, and to no less than 2^-32 of the largest that the row has.
  * scratch (16-byte boundary, ggb_kv8_attn_scratch_bytes; NULL: none) lets the keys of a few rows be spread over many CTAs. */
 size_t ggb_kv8_attn_scratch_bytes(int Dv);
