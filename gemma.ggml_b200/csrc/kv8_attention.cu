@@ -326,11 +326,11 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
         const int whole0 = s_it.kt + max(0, (down + Z::tile - 1) / Z::tile - s_it.w0), wholes = up < 0 ? 0 : max(0, s_it.kt + up / Z::tile - s_it.w0 - whole0 + 1);
 
         float rowf[NT][2], m[NT][2], l[NT][2], o[KS][NT][4];
-        int pow[NT][2]; // products of weights and scales are taken times 2^pow
+        int lift[NT][2]; // products of weights and scales are taken times 2^lift
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) rowf[t][e] = srow[8 * t + 2 * c4 + e], m[t][e] = kNone, l[t][e] = 0.f, pow[t][e] = 0;
+            for (int e = 0; e < 2; e++) rowf[t][e] = srow[8 * t + 2 * c4 + e], m[t][e] = kNone, l[t][e] = 0.f, lift[t][e] = 0;
 #pragma unroll
         for (int i = 0; i < KS; i++)
 #pragma unroll
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float most = m[t][e] + (float)min(8, kMostWeight - lv[u] - pow[t][e]);
+                        const float most = m[t][e] + (float)min(8, kMostWeight - lv[u] - lift[t][e]);
                         grow |= z[u][t][e] > most || z[u][t][e + 2] > most;
                     }
             }
@@ -466,9 +466,9 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                         for (int u = 0; u < Z::U; u++) p = fmaxf(p, (fmaxf(z[u][t][e], z[u][t][e + 2]) - x) + (float)lv[u]);
 #pragma unroll
                         for (int off = 4; off <= 16; off <<= 1) p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, off));
-                        const float d2 = (float)pow[t][e] + (x - m[t][e]), d = fminf(d2, (float)kNewWeight - ceilf(p)), f = exp2f(d - d2);
+                        const float d2 = (float)lift[t][e] + (x - m[t][e]), d = fminf(d2, (float)kNewWeight - ceilf(p)), f = exp2f(d - d2);
                         l[t][e] *= exp2f(m[t][e] - x);
-                        m[t][e] = x, pow[t][e] = (int)d;
+                        m[t][e] = x, lift[t][e] = (int)d;
 #pragma unroll
                         for (int i = 0; i < KS; i++) o[i][t][e] *= f, o[i][t][e + 2] *= f;
                     }
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
             for (int u = 0; u < Z::U; u++) {
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const float vrel[2] = {scale_times(sc[u].y, pow[t][0]), scale_times(sc[u].y, pow[t][1])};
+                    const float vrel[2] = {scale_times(sc[u].y, lift[t][0]), scale_times(sc[u].y, lift[t][1])};
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(step_sizes<CODE, P, NT, PARTS>::threads, step_
                 const int r = 8 * t + 2 * c4 + e;
 #pragma unroll
                 for (int off = 4; off <= 16; off <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], off);
-                if (g8 == 0) sm[warp * R + r] = m[t][e], sl[warp * R + r] = l[t][e], sd[warp * R + r] = (float)pow[t][e];
+                if (g8 == 0) sm[warp * R + r] = m[t][e], sl[warp * R + r] = l[t][e], sd[warp * R + r] = (float)lift[t][e];
                 float2 *row = red + (warp * R + r) * (P / 2);
 #pragma unroll
                 for (int i = 0; i < KS; i++) row[64 * (i / 8) + red_at<P>(g8, i % 8, c4)] = make_float2(o[i][t][e], o[i][t][e + 2]);
